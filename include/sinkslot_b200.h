@@ -353,6 +353,114 @@ int sinkslot_hvp(const float* x, const float* y, int d, const float* v, const fl
 int sinkslot_dual_value(const float* phi, const float* a, int64_t n, const float* psi,
                         const float* b, int64_t m, double* out, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Training operators (no counterpart in the reference): rows of a learned table
+ * that clouds are made of, token log-probabilities, and losses over them.
+ *
+ * dtype: 0 float32, 1 float16, 2 bfloat16.  Strides are in elements, from one
+ * row to the next; a row's own elements are contiguous and may begin on any
+ * element.  Sums, softmax statistics and means are held in fp32 or fp64; a
+ * result of 16 bits is rounded once.  None of the calls synchronises.
+ * ------------------------------------------------------------------------- */
+
+/* out[t, :] = scale * table[index[t], :], out (count, dim) contiguous; index
+ * int32 or int64 (index_bytes 4 or 8).  An index outside [0, rows) gives a row
+ * of NaN. */
+int sinkslot_lookup(const void* table, int dtype, int64_t stride, int64_t rows, int64_t dim,
+                    const void* index, int index_bytes, int64_t count, double scale, void* out,
+                    void* stream);
+
+int sinkslot_lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t dim,
+                                         int64_t* bytes_host);
+
+/* grad_table[v, :] = scale * sum of grad_out[t, :] over the t with index[t] = v,
+ * (rows, dim) contiguous; rows that no index names are zeros.  Tokens whose
+ * index is `padding` (-1: none) or outside [0, rows) give nothing.  The order of
+ * each sum follows from index alone. */
+int sinkslot_lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* index,
+                         int index_bytes, int64_t count, int64_t rows, int64_t dim, double scale,
+                         int64_t padding, void* grad_table, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* logp[r] = z[tok] - log sum_v exp z[v] with z = inv_temp * logits[r, :], and,
+ * where entropy is given, the entropy of softmax(z).  Rows whose token is
+ * `ignore` give 0 and are not read; a token outside [0, vocab) gives NaN; a row
+ * of -inf gives logp -inf and entropy 0.  stats (rows, 2) receives what the
+ * gradient needs: the row's maximum and its sum. */
+int sinkslot_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows,
+                            int64_t vocab, const void* tokens, int token_bytes, int64_t ignore,
+                            double inv_temp, float* logp, float* entropy, float* stats,
+                            void* stream);
+
+/* Gradient of the logits (same dtype, rows grad_stride apart) for the outer
+ * gradients g of logp and g_entropy of entropy (each nullable, not both; strides
+ * 0 or more).  entropy: the forward's output, needed with g_entropy. */
+int sinkslot_token_logprobs_grad(const void* logits, int dtype, int64_t stride, int64_t rows,
+                                 int64_t vocab, const void* tokens, int token_bytes,
+                                 int64_t ignore, double inv_temp, const float* stats,
+                                 const float* entropy, const float* g, int64_t g_stride,
+                                 const float* g_entropy, int64_t g_entropy_stride,
+                                 void* grad_logits, int64_t grad_stride, void* stream);
+
+int sinkslot_loss_workspace_bytes(int64_t sequences, int64_t* bytes_host);
+
+/* Clipped policy loss over packed sequences: with r = exp(logp - old_logp),
+ * -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * KL, averaged over
+ * the counted tokens (sequence_average 0) or over the means of the sequences
+ * that count a token (1).  offsets (sequences + 1 non-decreasing values, int32 or
+ * int64; null: one sequence of all tokens); mask (nullable, one byte per token;
+ * 0: not counted); advantages per token or per sequence; ref_logp nullable (no KL
+ * term); kl 1, 2, 3: with d = ref_logp - logp, -d, d^2 / 2, e^d - d - 1.
+ * values[0..3] = loss, mean KL, share of tokens clipped, norm; coef (nullable,
+ * tokens): d loss / d logp[t] = coef[t] * norm. */
+int sinkslot_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
+                         const float* advantages, int adv_per_token, const uint8_t* mask,
+                         const void* offsets, int offset_bytes, int64_t sequences, int64_t tokens,
+                         double clip_low, double clip_high, double kl_coef, int kl,
+                         int sequence_average, float* values, float* coef, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* out[t] = coef[t] * norm[0] * g[0] (16-byte aligned coef and out). */
+int sinkslot_scale_tokens(const float* coef, int64_t tokens, const float* norm, const float* g,
+                          float* out, void* stream);
+
+int sinkslot_policy_logits_workspace_bytes(int64_t rows, int64_t sequences, int64_t* bytes_host);
+
+/* sinkslot_policy_loss with logp taken from logits (as sinkslot_token_logprobs;
+ * rows with mask 0 give logp 0 and are not read), and, where grad_logits is
+ * given, the logits' gradient times grad_scale in the same call. */
+int sinkslot_policy_loss_logits(const void* logits, int dtype, int64_t stride, int64_t rows,
+                                int64_t vocab, const void* tokens, int token_bytes,
+                                double inv_temp, const float* old_logp, const float* ref_logp,
+                                const float* advantages, int adv_per_token, const uint8_t* mask,
+                                const void* offsets, int offset_bytes, int64_t sequences,
+                                double clip_low, double clip_high, double kl_coef, int kl,
+                                int sequence_average, double grad_scale, float* values,
+                                float* logp, void* grad_logits, int64_t grad_stride,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows of `grad` times g[0] / grad_scale, in place; nothing is touched where
+ * that is 1. */
+int sinkslot_scale_rows(void* grad, int dtype, int64_t stride, int64_t rows, int64_t vocab,
+                        const float* g, double grad_scale, void* stream);
+
+/* Preference loss over pairs of packed sequences: sequence i is chosen over
+ * sequence sequences / 2 + i.  R = sum over the counted tokens of logp - ref_logp
+ * (their mean with normalize), h = beta (R_chosen - R_rejected); kind 0:
+ * -(1 - smoothing) log sigma(h) - smoothing log sigma(-h), 1: max(0, 1 - h),
+ * 2: (h / beta - 1 / (2 beta))^2; loss[0] is the mean over the pairs.  rewards
+ * (sequences): beta R; slope (sequences): d loss / d logp of each counted token. */
+int sinkslot_preference_loss(const float* logp, const float* ref_logp, const uint8_t* mask,
+                             const void* offsets, int offset_bytes, int64_t sequences,
+                             int64_t tokens, double beta, double smoothing, int kind,
+                             int normalize, float* loss, float* rewards, float* slope,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[t] = slope of t's sequence * g[0] where t is counted, else 0. */
+int sinkslot_preference_grad(const float* slope, const uint8_t* mask, const void* offsets,
+                             int offset_bytes, int64_t sequences, int64_t tokens, const float* g,
+                             float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,6 +27,17 @@ from .gradient import (
 from .hvp import hvp_x_sqeuclid, hvp_x_sqeuclid_from_potentials
 from .samples_loss import SamplesLoss
 from .batched import sinkslot_solve_batched
+from .lookup import embedding_lookup
+from .logprobs import token_logprobs
+from .losses import (
+    PolicyLoss,
+    PolicyLossResult,
+    PreferenceLoss,
+    PreferenceLossResult,
+    policy_loss,
+    policy_loss_from_logits,
+    preference_loss,
+)
 from ._lib import LIB_PATH, SinkslotError, lib as load_library
 
 __all__ = [
@@ -45,6 +56,15 @@ __all__ = [
     "hvp_x_sqeuclid_from_potentials",
     "SamplesLoss",
     "sinkslot_solve_batched",
+    "embedding_lookup",
+    "token_logprobs",
+    "PolicyLoss",
+    "PolicyLossResult",
+    "PreferenceLoss",
+    "PreferenceLossResult",
+    "policy_loss",
+    "policy_loss_from_logits",
+    "preference_loss",
     "SinkslotError",
     "LIB_PATH",
     "load_library",

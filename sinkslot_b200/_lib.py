@@ -81,6 +81,27 @@ _SIGNATURES = {
     "sinkslot_barycentric": [c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_vp,
                              c_vp, c_vp, c_vp, c_i64, c_vp],
     "sinkslot_dual_value": [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp],
+    "sinkslot_lookup": [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_i64, c_dbl, c_vp, c_vp],
+    "sinkslot_lookup_grad_workspace_bytes": [c_i64, c_i64, c_i64, P_i64],
+    "sinkslot_lookup_grad": [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_dbl, c_i64,
+                             c_vp, c_vp, c_i64, c_vp],
+    "sinkslot_token_logprobs": [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_i64, c_dbl, c_vp,
+                                c_vp, c_vp, c_vp],
+    "sinkslot_token_logprobs_grad": [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_i64, c_dbl,
+                                     c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp],
+    "sinkslot_loss_workspace_bytes": [c_i64, P_i64],
+    "sinkslot_policy_loss": [c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_int, c_i64, c_i64, c_dbl,
+                             c_dbl, c_dbl, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_vp],
+    "sinkslot_scale_tokens": [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp],
+    "sinkslot_policy_logits_workspace_bytes": [c_i64, c_i64, P_i64],
+    "sinkslot_policy_loss_logits": [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_dbl, c_vp,
+                                    c_vp, c_vp, c_int, c_vp, c_vp, c_int, c_i64, c_dbl, c_dbl,
+                                    c_dbl, c_int, c_int, c_dbl, c_vp, c_vp, c_vp, c_i64, c_vp,
+                                    c_i64, c_vp],
+    "sinkslot_scale_rows": [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_dbl, c_vp],
+    "sinkslot_preference_loss": [c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_dbl, c_dbl, c_int,
+                                 c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
+    "sinkslot_preference_grad": [c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_vp],
     "sinkslot_hvp_workspace_bytes": [c_i64, c_i64, P_i64],
     "sinkslot_hvp": [c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
                      c_i64, c_i64, c_dbl, c_dbl, c_dbl, c_i64, c_vp, c_i64, c_vp, c_vp, P_i64,
@@ -143,3 +164,47 @@ def stream_of(device: torch.device) -> int:
 
 def out_i64() -> ctypes.c_int64:
     return ctypes.c_int64(0)
+
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def dtype_code(t: torch.Tensor) -> int:
+    return _DTYPES[t.dtype]
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_GUARD = _Here()
+
+
+def on_device(device: torch.device):
+    """A guard that makes ``device`` the current one (nothing where it is)."""
+    if device.index == torch.cuda.current_device():
+        return _HERE_GUARD
+    return torch.cuda.device(device)
+
+
+def require_cuda(name: str, *tensors: torch.Tensor) -> None:
+    dev = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"{name}: sinkslot_b200 runs on CUDA tensors only (got {t.device})")
+        if t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on one device")
+
+
+def require_dtype(name: str, what: str, t: torch.Tensor) -> None:
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name}: {what} must be float32, float16 or bfloat16, got {t.dtype}")
+
+
+def require_index(name: str, what: str, t: torch.Tensor) -> None:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")

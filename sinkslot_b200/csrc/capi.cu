@@ -9,6 +9,7 @@
 #include "primitives.h"
 #include "sinkhorn.h"
 #include "support.h"
+#include "training.h"
 
 namespace sinkslot {
 
@@ -35,7 +36,7 @@ extern "C" {
 
 const char* sinkslot_last_error(void) { return last_error(); }
 
-int sinkslot_abi_version(void) { return 101; }
+int sinkslot_abi_version(void) { return 102; }
 
 int sinkslot_project(const float* X, int64_t n, int d, const float* theta, int L, float* out,
                      void* stream) {
@@ -366,6 +367,183 @@ int sinkslot_dual_value(const float* phi, const float* a, int64_t n, const float
   SINKSLOT_REQUIRE(out && (n == 0 || (phi && a)) && (m == 0 || (psi && b)),
                    "dual_value: null argument");
   return dual_value(phi, a, n, psi, b, m, out, ST(stream));
+}
+
+
+int sinkslot_lookup(const void* table, int dtype, int64_t stride, int64_t rows, int64_t dim,
+                    const void* index, int index_bytes, int64_t count, double scale, void* out,
+                    void* stream) {
+  CAPI_BODY(lookup(table, dtype, stride, rows, dim, index, index_bytes, count, scale, out,
+                   ST(stream)));
+}
+
+int sinkslot_lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t dim,
+                                         int64_t* bytes_host) {
+  g_last_error_clear();
+  SINKSLOT_REQUIRE(bytes_host && count >= 0 && rows >= 1 && dim >= 1,
+                   "lookup_grad_workspace_bytes: bad args");
+  *bytes_host = (int64_t)lookup_grad_workspace_bytes(count, rows, dim);
+  return kOk;
+}
+
+int sinkslot_lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* index,
+                         int index_bytes, int64_t count, int64_t rows, int64_t dim, double scale,
+                         int64_t padding, void* grad_table, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  CAPI_BODY(lookup_grad(grad_out, dtype, stride, index, index_bytes, count, rows, dim, scale,
+                        padding, grad_table, workspace, (size_t)workspace_bytes, ST(stream)));
+}
+
+static LogitRows logit_rows(const void* logits, int dtype, int64_t stride, int64_t rows,
+                            int64_t vocab, const void* tokens, int token_bytes, int64_t ignore,
+                            double inv_temp) {
+  LogitRows r;
+  r.z = logits;
+  r.dtype = dtype;
+  r.stride = stride;
+  r.rows = rows;
+  r.vocab = vocab;
+  r.tokens = tokens;
+  r.token_bytes = token_bytes;
+  r.ignore = ignore;
+  r.inv_temp = inv_temp;
+  return r;
+}
+
+int sinkslot_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows,
+                            int64_t vocab, const void* tokens, int token_bytes, int64_t ignore,
+                            double inv_temp, float* logp, float* entropy, float* stats,
+                            void* stream) {
+  CAPI_BODY(token_logprobs(
+      logit_rows(logits, dtype, stride, rows, vocab, tokens, token_bytes, ignore, inv_temp), logp,
+      entropy, reinterpret_cast<float2*>(stats), ST(stream)));
+}
+
+int sinkslot_token_logprobs_grad(const void* logits, int dtype, int64_t stride, int64_t rows,
+                                 int64_t vocab, const void* tokens, int token_bytes,
+                                 int64_t ignore, double inv_temp, const float* stats,
+                                 const float* entropy, const float* g, int64_t g_stride,
+                                 const float* g_entropy, int64_t g_entropy_stride,
+                                 void* grad_logits, int64_t grad_stride, void* stream) {
+  LogitGrad q;
+  q.g = g;
+  q.g_stride = g_stride;
+  q.g_entropy = g_entropy;
+  q.g_entropy_stride = g_entropy_stride;
+  q.entropy = entropy;
+  q.stats = reinterpret_cast<const float2*>(stats);
+  q.dz = grad_logits;
+  q.dz_stride = grad_stride;
+  CAPI_BODY(token_logprobs_grad(
+      logit_rows(logits, dtype, stride, rows, vocab, tokens, token_bytes, ignore, inv_temp), q,
+      ST(stream)));
+}
+
+int sinkslot_loss_workspace_bytes(int64_t sequences, int64_t* bytes_host) {
+  g_last_error_clear();
+  SINKSLOT_REQUIRE(bytes_host && sequences >= 1, "loss_workspace_bytes: bad args");
+  *bytes_host = (int64_t)loss_workspace_bytes(sequences);
+  return kOk;
+}
+
+static Packed packed(const uint8_t* mask, const void* offsets, int offset_bytes, int64_t sequences,
+                     int64_t tokens) {
+  Packed p;
+  p.tokens = tokens;
+  p.offsets = offsets;
+  p.offset_bytes = offset_bytes;
+  p.count = sequences;
+  p.mask = mask;
+  return p;
+}
+
+static PolicyTerms policy_terms(const float* logp, const float* old_logp, const float* ref_logp,
+                                const float* advantages, int adv_per_token, double clip_low,
+                                double clip_high, double kl_coef, int kl, int sequence_average) {
+  PolicyTerms t;
+  t.logp = logp;
+  t.old_logp = old_logp;
+  t.ref_logp = ref_logp;
+  t.adv = advantages;
+  t.adv_per_token = adv_per_token;
+  t.clip_low = clip_low;
+  t.clip_high = clip_high;
+  t.kl_coef = kl_coef;
+  t.kl_kind = kl;
+  t.sequence_average = sequence_average;
+  return t;
+}
+
+int sinkslot_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
+                         const float* advantages, int adv_per_token, const uint8_t* mask,
+                         const void* offsets, int offset_bytes, int64_t sequences, int64_t tokens,
+                         double clip_low, double clip_high, double kl_coef, int kl,
+                         int sequence_average, float* values, float* coef, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  CAPI_BODY(policy_loss(packed(mask, offsets, offset_bytes, sequences, tokens),
+                        policy_terms(logp, old_logp, ref_logp, advantages, adv_per_token, clip_low,
+                                     clip_high, kl_coef, kl, sequence_average),
+                        values, coef, workspace, (size_t)workspace_bytes, ST(stream)));
+}
+
+int sinkslot_scale_tokens(const float* coef, int64_t tokens, const float* norm, const float* g,
+                          float* out, void* stream) {
+  CAPI_BODY(scale_tokens(coef, tokens, norm, g, out, ST(stream)));
+}
+
+int sinkslot_policy_logits_workspace_bytes(int64_t rows, int64_t sequences, int64_t* bytes_host) {
+  g_last_error_clear();
+  SINKSLOT_REQUIRE(bytes_host && rows >= 0 && sequences >= 1,
+                   "policy_logits_workspace_bytes: bad args");
+  *bytes_host = (int64_t)policy_logits_workspace_bytes(rows, sequences);
+  return kOk;
+}
+
+int sinkslot_policy_loss_logits(const void* logits, int dtype, int64_t stride, int64_t rows,
+                                int64_t vocab, const void* tokens, int token_bytes,
+                                double inv_temp, const float* old_logp, const float* ref_logp,
+                                const float* advantages, int adv_per_token, const uint8_t* mask,
+                                const void* offsets, int offset_bytes, int64_t sequences,
+                                double clip_low, double clip_high, double kl_coef, int kl,
+                                int sequence_average, double grad_scale, float* values,
+                                float* logp, void* grad_logits, int64_t grad_stride,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
+  LogitRows r = logit_rows(logits, dtype, stride, rows, vocab, tokens, token_bytes, INT64_MIN,
+                           inv_temp);
+  r.mask = mask;
+  CAPI_BODY(policy_loss_logits(r, packed(mask, offsets, offset_bytes, sequences, rows),
+                               policy_terms(nullptr, old_logp, ref_logp, advantages, adv_per_token,
+                                            clip_low, clip_high, kl_coef, kl, sequence_average),
+                               (float)grad_scale, values, logp, grad_logits, grad_stride,
+                               workspace, (size_t)workspace_bytes, ST(stream)));
+}
+
+int sinkslot_scale_rows(void* grad, int dtype, int64_t stride, int64_t rows, int64_t vocab,
+                        const float* g, double grad_scale, void* stream) {
+  CAPI_BODY(scale_rows(grad, dtype, stride, rows, vocab, g, (float)grad_scale, ST(stream)));
+}
+
+int sinkslot_preference_loss(const float* logp, const float* ref_logp, const uint8_t* mask,
+                             const void* offsets, int offset_bytes, int64_t sequences,
+                             int64_t tokens, double beta, double smoothing, int kind,
+                             int normalize, float* loss, float* rewards, float* slope,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  PreferenceTerms t;
+  t.logp = logp;
+  t.ref_logp = ref_logp;
+  t.beta = beta;
+  t.smoothing = smoothing;
+  t.kind = kind;
+  t.normalize = normalize;
+  CAPI_BODY(preference_loss(packed(mask, offsets, offset_bytes, sequences, tokens), t, loss,
+                            rewards, slope, workspace, (size_t)workspace_bytes, ST(stream)));
+}
+
+int sinkslot_preference_grad(const float* slope, const uint8_t* mask, const void* offsets,
+                             int offset_bytes, int64_t sequences, int64_t tokens, const float* g,
+                             float* out, void* stream) {
+  CAPI_BODY(preference_grad(packed(mask, offsets, offset_bytes, sequences, tokens), slope, g, out,
+                            ST(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,484 @@
+// losses.cu -- losses over the log-probabilities of packed sequences, with the
+// gradient of each token.
+//
+//   policy      r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta KL,
+//               averaged over the counted tokens, or over the sequences' means;
+//               KL from d = ref - logp: k1 -d, k2 d^2 / 2, k3 e^d - d - 1
+//   preference  R_i = sum_t (logp - ref) (or its mean), h = beta (R_chosen - R_rejected),
+//               -(1 - ls) log sigma(h) - ls log sigma(-h), max(0, 1 - h), or
+//               (h / beta - 1 / (2 beta))^2, averaged over the pairs
+//
+// Both read a few bytes for each token: launch latency bounds the ordinary
+// sizes.  A cluster of CTAs takes a sequence (8 of them where there are few),
+// its sums are joined in a fixed order in fp64, and one CTA, launched so that it
+// starts while the first kernel ends, joins the sequences.
+#include <cmath>
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "training.h"
+
+namespace sinkslot {
+
+namespace cg = cooperative_groups;
+
+constexpr int kLossThreads = 512;
+constexpr int kLossWarps = kLossThreads / 32;
+constexpr int kLossSplit = 8;
+
+struct Sums {
+  double a, b, c;
+};
+
+// Sums over the CTA's threads and the cluster's CTAs, in a fixed order; every
+// thread of the cluster gets them.  `turn` alternates between consecutive calls.
+struct ClusterSum {
+  Sums warp[kLossWarps];
+  Sums cta[2][kLossSplit];
+};
+
+__device__ __forceinline__ Sums warp_sums(Sums v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    v.a += __shfl_xor_sync(0xffffffffu, v.a, o);
+    v.b += __shfl_xor_sync(0xffffffffu, v.b, o);
+    v.c += __shfl_xor_sync(0xffffffffu, v.c, o);
+  }
+  return v;
+}
+
+__device__ __forceinline__ Sums cluster_sums(Sums v, ClusterSum& sh, int turn, int rank,
+                                             int split) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_sums(v);
+  __syncthreads();
+  if (lane == 0) sh.warp[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    const Sums zero = {0.0, 0.0, 0.0};
+    v = warp_sums(lane < kLossWarps ? sh.warp[lane] : zero);
+    if (lane < split) {
+      if (split > 1)
+        cg::this_cluster().map_shared_rank(&sh.cta[turn][0], lane)[rank] = v;
+      else
+        sh.cta[turn][0] = v;
+    }
+  }
+  if (split > 1)
+    cg::this_cluster().sync();
+  else
+    __syncthreads();
+  Sums t = {0.0, 0.0, 0.0};
+  for (int k = 0; k < split; ++k) {
+    t.a += sh.cta[turn][k].a;
+    t.b += sh.cta[turn][k].b;
+    t.c += sh.cta[turn][k].c;
+  }
+  return t;
+}
+
+// Bounds of sequence i, kept within the tokens whatever the offsets hold.
+__device__ __forceinline__ int64_t offset_at(const Packed& p, int64_t i) {
+  int64_t v = p.offset_bytes == 8 ? static_cast<const int64_t*>(p.offsets)[i]
+                                  : (int64_t) static_cast<const int32_t*>(p.offsets)[i];
+  v = v < 0 ? 0 : v;
+  return v > p.tokens ? p.tokens : v;
+}
+__device__ __forceinline__ void bounds(const Packed& p, int64_t i, int64_t& lo, int64_t& hi) {
+  lo = p.offsets ? offset_at(p, i) : 0;
+  hi = p.offsets ? offset_at(p, i + 1) : p.tokens;
+  if (hi < lo) hi = lo;
+}
+
+// Zeros for the tokens before the first sequence and behind the last.
+__device__ __forceinline__ void zero_outside(const Packed& p, int64_t seq, int64_t at, int64_t step,
+                                             float* out) {
+  if (!p.offsets || !out) return;
+  if (seq == 0)
+    for (int64_t t = at, e = offset_at(p, 0); t < e; t += step) out[t] = 0.0f;
+  if (seq == p.count - 1)
+    for (int64_t t = offset_at(p, p.count) + at; t < p.tokens; t += step) out[t] = 0.0f;
+}
+
+// e^d - d - 1.  Near 0 its terms cancel; there it is summed as its series
+// d^2/2! + d^3/3! + ... + d^11/11! (the rest is under 2^-30 of it for |d| <= 1/2).
+__device__ __forceinline__ float exp_gap(float d) {
+  if (d >= 1e4f) return INFINITY;
+  if (!(fabsf(d) <= 0.5f)) return expm1f(d) - d;
+  float t = 1.0f;
+#pragma unroll
+  for (int k = 11; k >= 3; --k) t = fmaf(t, d * (1.0f / (float)k), 1.0f);
+  return 0.5f * d * d * t;
+}
+
+struct PolicyEdges {
+  double under, over;  // log(1 - lo), log(1 + hi)
+  float rlo, rhi, kl_coef;
+};
+
+struct TokenTerm {
+  float loss, kl, coef;
+  bool clipped;
+};
+
+// One token's loss, KL estimate and d loss / d logp.  The clip is decided on the
+// difference of the log-probabilities in fp64, which is exact.
+__device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
+                                                 float logp, int64_t at, int64_t seq) {
+  TokenTerm o;
+  const double d = (double)logp - (double)t.old_logp[at];
+  const float adv = t.adv[t.adv_per_token ? at : seq];
+  const bool over = d > e.over, under = d < e.under;
+  const float r = expf((float)d);
+  const float rc = over ? e.rhi : (under ? e.rlo : r);
+  // min(r A, clip(r) A) is the clipped one where r is outside on A's side
+  o.clipped = adv > 0.0f ? over : (adv < 0.0f ? under : false);
+  o.loss = -(o.clipped ? rc : r) * adv;
+  o.coef = o.clipped ? 0.0f : -r * adv;
+  o.kl = 0.0f;
+  if (t.ref_logp) {
+    const float g = (float)((double)t.ref_logp[at] - (double)logp);
+    float slope;
+    if (t.kl_kind == 1) {
+      o.kl = -g;
+      slope = 1.0f;
+    } else if (t.kl_kind == 2) {
+      o.kl = 0.5f * g * g;
+      slope = -g;
+    } else {
+      o.kl = exp_gap(g);
+      slope = -expm1f(g);
+    }
+    if (e.kl_coef != 0.0f) {
+      o.loss = fmaf(e.kl_coef, o.kl, o.loss);
+      o.coef = fmaf(e.kl_coef, slope, o.coef);
+    }
+  }
+  return o;
+}
+
+static PolicyEdges policy_edges(const PolicyTerms& t) {
+  PolicyEdges e;
+  e.under = t.clip_low >= 1.0 ? -INFINITY : log1p(-t.clip_low);
+  e.over = log1p(t.clip_high);
+  e.rlo = t.clip_low >= 1.0 ? 0.0f : (float)(1.0 - t.clip_low);
+  e.rhi = (float)(1.0 + t.clip_high);
+  e.kl_coef = (float)t.kl_coef;
+  return e;
+}
+
+// Per sequence: {loss, kl, clipped, counted}.
+__global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, PolicyTerms t,
+                                                                  PolicyEdges e, int split,
+                                                                  double4* __restrict__ part,
+                                                                  float* __restrict__ coef) {
+  __shared__ ClusterSum sh;
+  const int64_t seq = blockIdx.x / (unsigned)split;
+  const int rank = (int)(blockIdx.x % (unsigned)split);
+  const int64_t at = (int64_t)rank * kLossThreads + threadIdx.x;
+  const int64_t step = (int64_t)split * kLossThreads;
+  int64_t lo, hi;
+  bounds(p, seq, lo, hi);
+  double inv = 1.0;
+  if (t.sequence_average) {
+    double n = (double)(hi - lo);
+    if (p.mask) {
+      int64_t k = 0;
+      for (int64_t i = lo + at; i < hi; i += step) k += p.mask[i] != 0;
+      n = cluster_sums({(double)k, 0.0, 0.0}, sh, 0, rank, split).a;
+    }
+    inv = n > 0.0 ? 1.0 / n : 0.0;
+  }
+  const float finv = (float)inv;
+  Sums s = {0.0, 0.0, 0.0};
+  int64_t n = 0;
+  for (int64_t i = lo + at; i < hi; i += step) {
+    float cf = 0.0f;
+    if (!p.mask || p.mask[i]) {
+      const TokenTerm o = policy_term(t, e, t.logp[i], i, seq);
+      s.a += (double)o.loss;
+      s.b += (double)o.kl;
+      n += 1 + ((int64_t)o.clipped << 32);
+      cf = o.coef * finv;
+    }
+    if (coef) coef[i] = cf;
+  }
+  zero_outside(p, seq, at, step, coef);
+  // counts of counted and of clipped tokens, both under 2^32, apart in fp64
+  s.c = (double)(n & 0xffffffff);
+  const Sums f = cluster_sums(s, sh, 1, rank, split);
+  const Sums k = cluster_sums({(double)(n >> 32), 0.0, 0.0}, sh, 0, rank, split);
+  if (rank == 0 && threadIdx.x == 0) part[seq] = make_double4(f.a * inv, f.b * inv, k.a, f.c);
+  chain_release();
+}
+
+// Sums over one CTA of kLossThreads (no cluster).
+__device__ __forceinline__ Sums cta_sums(Sums v, ClusterSum& sh, int turn) {
+  return cluster_sums(v, sh, turn, 0, 1);
+}
+
+__global__ void __launch_bounds__(kLossThreads) policy_end_kernel(const double4* __restrict__ part,
+                                                                  int64_t count, int by_sequence,
+                                                                  float* __restrict__ values) {
+  __shared__ ClusterSum sh;
+  chain_enter();
+  Sums s = {0.0, 0.0, 0.0}, k = {0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < count; i += kLossThreads) {
+    const double4 v = part[i];
+    s.a += v.x;
+    s.b += v.y;
+    s.c += v.z;
+    k.a += v.w;
+    k.b += v.w > 0.0 ? 1.0 : 0.0;
+  }
+  s = cta_sums(s, sh, 0);
+  k = cta_sums(k, sh, 1);
+  if (threadIdx.x == 0) {
+    const double over = by_sequence ? k.b : k.a;
+    const double norm = over > 0.0 ? 1.0 / over : 0.0;
+    values[0] = (float)(s.a * norm);
+    values[1] = (float)(s.b * norm);
+    values[2] = k.a > 0.0 ? (float)(s.c / k.a) : 0.0f;
+    values[3] = (float)norm;
+  }
+}
+
+// CTAs for each sequence: a cluster of 8 while the sequences do not fill the
+// GPU, each with 1024 tokens of an average sequence or more.
+static int loss_split(const Packed& p) {
+  int split = 1;
+  while (split < kLossSplit && p.count * split * 2 <= 2 * num_sms() &&
+         p.tokens / p.count >= (int64_t)split * 2 * 1024)
+    split *= 2;
+  return split;
+}
+
+template <typename... Params, typename... Args>
+static cudaError_t launch_cluster(void (*kernel)(Params...), int64_t count, int split, int threads,
+                                  cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(count * split));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+static int check_packed(const Packed& p) {
+  SINKSLOT_REQUIRE(p.tokens >= 0 && p.count >= 1 && p.count <= (int64_t(1) << 27),
+                   "loss: bad sizes");
+  SINKSLOT_REQUIRE(p.tokens < (int64_t(1) << 32), "loss: 2^32 tokens or more");
+  SINKSLOT_REQUIRE(p.offsets || p.count == 1, "loss: offsets are required");
+  SINKSLOT_REQUIRE(p.offset_bytes == 4 || p.offset_bytes == 8, "loss: offsets int32 or int64");
+  return kOk;
+}
+
+size_t loss_workspace_bytes(int64_t count) {
+  return align_up((size_t)(count > 0 ? count : 1) * sizeof(double4));
+}
+
+int policy_loss(const Packed& p, const PolicyTerms& t, float* values, float* coef, void* ws,
+                size_t ws_bytes, cudaStream_t st) {
+  SINKSLOT_TRY(check_packed(p));
+  SINKSLOT_REQUIRE(values && ws, "policy_loss: null argument");
+  SINKSLOT_REQUIRE(p.tokens == 0 || (t.logp && t.old_logp && t.adv), "policy_loss: null argument");
+  SINKSLOT_REQUIRE(t.clip_low >= 0.0 && t.clip_high >= 0.0, "policy_loss: clip must be >= 0");
+  SINKSLOT_REQUIRE(t.kl_kind >= 1 && t.kl_kind <= 3, "policy_loss: kl must be 1, 2 or 3");
+  if (ws_bytes < loss_workspace_bytes(p.count)) {
+    set_error("policy_loss: workspace too small");
+    return kWorkspaceTooSmall;
+  }
+  double4* part = static_cast<double4*>(ws);
+  const int split = loss_split(p);
+  SINKSLOT_CUDA_TRY(launch_cluster(policy_seq_kernel, p.count, split, kLossThreads, st, p, t,
+                                   policy_edges(t), split, part, coef));
+  SINKSLOT_CUDA_TRY(launch_chained(policy_end_kernel, dim3(1), dim3(kLossThreads), 0, st,
+                                   (const double4*)part, p.count, t.sequence_average, values));
+  return kOk;
+}
+
+// --------------------------------------------------------------------------
+// Preference loss
+// --------------------------------------------------------------------------
+__global__ void __launch_bounds__(kLossThreads) preference_seq_kernel(
+    Packed p, const float* __restrict__ logp, const float* __restrict__ ref, int split,
+    double2* __restrict__ part) {
+  __shared__ ClusterSum sh;
+  const int64_t seq = blockIdx.x / (unsigned)split;
+  const int rank = (int)(blockIdx.x % (unsigned)split);
+  int64_t lo, hi;
+  bounds(p, seq, lo, hi);
+  Sums s = {0.0, 0.0, 0.0};
+  int64_t n = 0;
+  for (int64_t i = lo + (int64_t)rank * kLossThreads + threadIdx.x; i < hi;
+       i += (int64_t)split * kLossThreads) {
+    if (p.mask && !p.mask[i]) continue;
+    s.a += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
+    ++n;
+  }
+  s.b = (double)n;
+  const Sums f = cluster_sums(s, sh, 0, rank, split);
+  if (rank == 0 && threadIdx.x == 0) part[seq] = make_double2(f.a, f.b);
+  chain_release();
+}
+
+__global__ void __launch_bounds__(kLossThreads) preference_end_kernel(
+    const double2* __restrict__ part, int64_t pairs, double beta, double smoothing, int kind,
+    int normalize, float* __restrict__ loss, float* __restrict__ rewards,
+    float* __restrict__ slope) {
+  __shared__ ClusterSum sh;
+  chain_enter();
+  Sums s = {0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < pairs; i += kLossThreads) {
+    const double2 c = part[i], r = part[pairs + i];
+    const double wc = normalize && c.y > 0.0 ? 1.0 / c.y : 1.0;
+    const double wr = normalize && r.y > 0.0 ? 1.0 / r.y : 1.0;
+    const double rc = beta * c.x * wc, rr = beta * r.x * wr;
+    const double h = rc - rr;
+    double each, d;  // the pair's loss and its derivative by h
+    if (kind == 0) {
+      const double u = exp(-fabs(h));           // sigma(-|h|) = u / (1 + u)
+      const double soft = log1p(u);
+      const double neg = (h > 0.0 ? u : 1.0) / (1.0 + u), pos = (h > 0.0 ? 1.0 : u) / (1.0 + u);
+      each = (1.0 - smoothing) * (soft + (h < 0.0 ? -h : 0.0)) +
+             smoothing * (soft + (h > 0.0 ? h : 0.0));
+      if (h != h) each = h;
+      d = smoothing * pos - (1.0 - smoothing) * neg;
+    } else if (kind == 1) {
+      each = h < 1.0 ? 1.0 - h : 0.0;
+      if (h != h) each = h;
+      d = h < 1.0 ? -1.0 : 0.0;
+    } else {
+      const double x = h / beta - 0.5 / beta;
+      each = x * x;
+      d = 2.0 * x / beta;
+    }
+    s.a += each;
+    d *= beta / (double)pairs;
+    rewards[i] = (float)rc;
+    rewards[pairs + i] = (float)rr;
+    slope[i] = (float)(d * wc);
+    slope[pairs + i] = (float)(-d * wr);
+  }
+  s = cta_sums(s, sh, 0);
+  if (threadIdx.x == 0) loss[0] = (float)(s.a / (double)pairs);
+}
+
+int preference_loss(const Packed& p, const PreferenceTerms& t, float* loss, float* rewards,
+                    float* slope, void* ws, size_t ws_bytes, cudaStream_t st) {
+  SINKSLOT_TRY(check_packed(p));
+  SINKSLOT_REQUIRE(p.offsets && p.count % 2 == 0, "preference_loss: sequences come in pairs");
+  SINKSLOT_REQUIRE(loss && rewards && slope && ws && (p.tokens == 0 || t.logp),
+                   "preference_loss: null argument");
+  SINKSLOT_REQUIRE(t.kind >= 0 && t.kind <= 2 && t.beta > 0.0, "preference_loss: bad args");
+  if (ws_bytes < loss_workspace_bytes(p.count)) {
+    set_error("preference_loss: workspace too small");
+    return kWorkspaceTooSmall;
+  }
+  double2* part = static_cast<double2*>(ws);
+  const int split = loss_split(p);
+  SINKSLOT_CUDA_TRY(launch_cluster(preference_seq_kernel, p.count, split, kLossThreads, st, p,
+                                   t.logp, t.ref_logp, split, part));
+  SINKSLOT_CUDA_TRY(launch_chained(preference_end_kernel, dim3(1), dim3(kLossThreads), 0, st,
+                                   (const double2*)part, p.count / 2, t.beta, t.smoothing, t.kind,
+                                   t.normalize, loss, rewards, slope));
+  return kOk;
+}
+
+__global__ void __launch_bounds__(kLossThreads) preference_grad_kernel(
+    Packed p, const float* __restrict__ slope, const float* __restrict__ g, int split,
+    float* __restrict__ out) {
+  const int64_t seq = blockIdx.x / (unsigned)split;
+  const int64_t at = (int64_t)(blockIdx.x % (unsigned)split) * kLossThreads + threadIdx.x;
+  const int64_t step = (int64_t)split * kLossThreads;
+  int64_t lo, hi;
+  bounds(p, seq, lo, hi);
+  const float v = slope[seq] * g[0];
+  for (int64_t i = lo + at; i < hi; i += step) out[i] = !p.mask || p.mask[i] ? v : 0.0f;
+  zero_outside(p, seq, at, step, out);
+}
+
+int preference_grad(const Packed& p, const float* slope, const float* g, float* out,
+                    cudaStream_t st) {
+  SINKSLOT_TRY(check_packed(p));
+  if (p.tokens == 0) return kOk;
+  SINKSLOT_REQUIRE(slope && g && out, "preference_grad: null argument");
+  const int split = loss_split(p);
+  preference_grad_kernel<<<(unsigned)(p.count * split), kLossThreads, 0, st>>>(p, slope, g, split,
+                                                                              out);
+  SINKSLOT_CHECK_LAUNCH();
+  return kOk;
+}
+
+__global__ void __launch_bounds__(256) scale_tokens_kernel(const float* __restrict__ coef,
+                                                           int64_t tokens,
+                                                           const float* __restrict__ norm,
+                                                           const float* __restrict__ g,
+                                                           float* __restrict__ out) {
+  const float f = norm[0] * g[0];
+  const int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i0 + 4 <= tokens) {
+    float4 v = reinterpret_cast<const float4*>(coef)[i0 / 4];
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    reinterpret_cast<float4*>(out)[i0 / 4] = v;
+  } else {
+    for (int64_t i = i0; i < tokens; ++i) out[i] = coef[i] * f;
+  }
+}
+
+int scale_tokens(const float* coef, int64_t tokens, const float* norm, const float* g, float* out,
+                 cudaStream_t st) {
+  SINKSLOT_REQUIRE(tokens >= 0, "scale_tokens: bad sizes");
+  if (tokens == 0) return kOk;
+  SINKSLOT_REQUIRE(coef && norm && g && out, "scale_tokens: null argument");
+  SINKSLOT_REQUIRE(((reinterpret_cast<uintptr_t>(coef) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+                   "scale_tokens: 16-byte alignment is required");
+  scale_tokens_kernel<<<(unsigned)ceil_div64(tokens, 1024), 256, 0, st>>>(coef, tokens, norm, g,
+                                                                         out);
+  SINKSLOT_CHECK_LAUNCH();
+  return kOk;
+}
+
+// --------------------------------------------------------------------------
+// Policy loss from the logits: log-probabilities, token terms, logits' gradient.
+// --------------------------------------------------------------------------
+size_t policy_logits_workspace_bytes(int64_t rows, int64_t count) {
+  const size_t r = (size_t)(rows > 0 ? rows : 1);
+  return loss_workspace_bytes(count) + align_up(r * sizeof(float2)) + align_up(r * sizeof(float));
+}
+
+int policy_loss_logits(const LogitRows& r, const Packed& p, const PolicyTerms& t, float grad_scale,
+                       float* values, float* logp, void* dz, int64_t dz_stride, void* ws,
+                       size_t ws_bytes, cudaStream_t st) {
+  SINKSLOT_REQUIRE(p.tokens == r.rows, "policy_loss_from_logits: bad sizes");
+  Carver cv(ws, ws_bytes);
+  float2* stats = cv.take<float2>((size_t)(r.rows > 0 ? r.rows : 1));
+  float* coef = cv.take<float>((size_t)(r.rows > 0 ? r.rows : 1));
+  char* part = cv.take<char>(loss_workspace_bytes(p.count));
+  if (!cv.ok) {
+    set_error("policy_loss_from_logits: workspace too small");
+    return kWorkspaceTooSmall;
+  }
+  SINKSLOT_TRY(token_logprobs(r, logp, nullptr, stats, st));
+  PolicyTerms u = t;
+  u.logp = logp;
+  SINKSLOT_TRY(policy_loss(p, u, values, dz ? coef : nullptr, part, loss_workspace_bytes(p.count),
+                           st));
+  if (!dz || r.rows == 0) return kOk;
+  LogitGrad g;
+  g.g = coef;
+  g.g_stride = 1;
+  g.scale_dev = values + 3;
+  g.scale = grad_scale;
+  g.stats = stats;
+  g.dz = dz;
+  g.dz_stride = dz_stride;
+  return token_logprobs_grad(r, g, st);
+}
+
+}  // namespace sinkslot
