@@ -38,7 +38,7 @@ from .losses import (
     policy_loss_from_logits,
     preference_loss,
 )
-from ._lib import LIB_PATH, SinkslotError, lib as load_library
+from ._lib import LIB_PATH, SinkslotError, load_library
 
 __all__ = [
     "get_random_projections",
@@ -69,3 +69,8 @@ __all__ = [
     "LIB_PATH",
     "load_library",
 ]
+
+try:  # registers the training operators too, where they are built (else at the first use)
+    load_library()
+except (ImportError, OSError):
+    pass

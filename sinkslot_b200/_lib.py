@@ -10,11 +10,13 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+import types
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsinkslot_b200.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "libsinkslot_b200_torch.so")
 
 _lock = threading.Lock()
 _lib = None
@@ -166,45 +168,33 @@ def out_i64() -> ctypes.c_int64:
     return ctypes.c_int64(0)
 
 
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_torch_ops = None
 
 
-def dtype_code(t: torch.Tensor) -> int:
-    return _DTYPES[t.dtype]
+def torch_ops():
+    """The training operators that users' functions call, from
+    libsinkslot_b200_torch.so; raises if it is missing (no fallback exists)."""
+    global _torch_ops
+    if _torch_ops is not None:
+        return _torch_ops
+    lib()
+    with _lock:
+        if _torch_ops is None:
+            if not os.path.exists(TORCH_LIB_PATH):
+                raise ImportError(
+                    f"{TORCH_LIB_PATH} is missing: the training operators must be built "
+                    f"(python -m sinkslot_b200.build); sinkslot_b200 has no fallback")
+            torch.ops.load_library(TORCH_LIB_PATH)
+            from . import ops
+            ops.register_training_fakes()
+            ns = torch.ops.sinkslot_b200
+            _torch_ops = types.SimpleNamespace(
+                **{n: getattr(ns, n).default for n in ("embedding_lookup", "logprobs", "policy",
+                                                       "policy_from_logits", "preference")})
+    return _torch_ops
 
 
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_GUARD = _Here()
-
-
-def on_device(device: torch.device):
-    """A guard that makes ``device`` the current one (nothing where it is)."""
-    if device.index == torch.cuda.current_device():
-        return _HERE_GUARD
-    return torch.cuda.device(device)
-
-
-def require_cuda(name: str, *tensors: torch.Tensor) -> None:
-    dev = tensors[0].device
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"{name}: sinkslot_b200 runs on CUDA tensors only (got {t.device})")
-        if t.device != dev:
-            raise ValueError(f"{name}: all tensors must be on one device")
-
-
-def require_dtype(name: str, what: str, t: torch.Tensor) -> None:
-    if t.dtype not in _DTYPES:
-        raise ValueError(f"{name}: {what} must be float32, float16 or bfloat16, got {t.dtype}")
-
-
-def require_index(name: str, what: str, t: torch.Tensor) -> None:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")
+def load_library():
+    """Loads both libraries now; the C ABI's binding is returned."""
+    torch_ops()
+    return lib()

@@ -4,7 +4,9 @@
 ``sm_100a`` and links them into ``sinkslot_b200/libsinkslot_b200.so`` (static
 cudart, C ABI declared in ``include/sinkslot_b200.h``).  Objects go to
 ``sinkslot_b200/_build/``; sources are rebuilt only when they, or a header,
-changed.
+changed.  ``csrc/torch_ops.cpp`` (the training operators' PyTorch bindings, host
+code only) becomes ``sinkslot_b200/libsinkslot_b200_torch.so``, linked to that
+library and to the installed torch.
 """
 
 from __future__ import annotations
@@ -21,6 +23,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsinkslot_b200.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_LIB = os.path.join(HERE, "libsinkslot_b200_torch.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -40,6 +44,35 @@ def _headers_mtime() -> float:
     hs = glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh"))
     hs += glob.glob(os.path.join(ROOT, "include", "*.h"))
     return max((os.path.getmtime(h) for h in hs), default=0.0)
+
+
+def _build_torch_ops(verbose: bool) -> None:
+    """libsinkslot_b200_torch.so, when its source, the C header or torch changed."""
+    import torch
+    stamp = os.path.join(BUILD, "torch_version")
+    header = os.path.join(ROOT, "include", "sinkslot_b200.h")
+    if os.path.exists(TORCH_LIB) and os.path.exists(stamp):
+        newest = max(os.path.getmtime(TORCH_SRC), os.path.getmtime(header))
+        if os.path.getmtime(TORCH_LIB) >= newest and open(stamp).read() == torch.__version__:
+            return
+    t = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    tmp = f"{TORCH_LIB}.{os.getpid()}.tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(t, "include"),
+           "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), TORCH_SRC, "-o", tmp,
+           "-L" + HERE, "-l:" + os.path.basename(LIB), "-L" + os.path.join(t, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for csrc/torch_ops.cpp")
+    os.replace(tmp, TORCH_LIB)
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
 
 
 def build(verbose: bool = False, ptxas_info: bool = False) -> str:
@@ -75,6 +108,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
             raise RuntimeError("link of libsinkslot_b200.so failed")
         os.replace(tmp, LIB)
+    _build_torch_ops(verbose)
     return LIB
 
 

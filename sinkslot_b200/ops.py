@@ -6,11 +6,13 @@ these operators, so the calls are visible to PyTorch's dispatcher, profiler and
 shapes without running anything; the support's size is data-dependent and is a
 dynamic size there).  The operator bodies are the host wrappers of the C ABI;
 none has a CPU kernel: the library runs on CUDA tensors only.
+
+The training operators' bodies are C++ (``csrc/torch_ops.cpp``); only their fake
+implementations are here.
 """
 
 from __future__ import annotations
 
-import importlib
 from typing import Optional
 
 import torch
@@ -130,66 +132,33 @@ def _(X, Y, a, v, rows, cols, T_vals, eps, tau2, solve_tol, max_cg_iter):
     return X.new_empty(X.shape), torch.empty(2, dtype=torch.float64, device="cpu")
 
 
-# The training operators: called many times a step on small tensors too, so they
-# are defined with the lighter of the library's two registrations (measured: the
-# custom_op wrapper adds 20 us of host time to a call).
-_training = torch.library.Library(NS, "FRAGMENT")
-
-
-def _define(schema: str, where: str, body: str, fake) -> None:
-    """Registers an operator whose CUDA body is ``where.body`` (imported at the first call)."""
-    name = schema.split("(", 1)[0]
-    _training.define(schema)
-    found = []
-
-    def run(*args):
-        if not found:
-            found.append(getattr(importlib.import_module(f"{__package__}.{where}"), body))
-        return found[0](*args)
-
-    _training.impl(name, run, "CUDA")
-    torch.library.register_fake(f"{NS}::{name}", fake)
-
-
 def _f32(like, *shape):
     return like.new_empty(shape, dtype=torch.float32)
 
 
-_define("lookup(Tensor table, Tensor index, float scale) -> Tensor", "lookup", "_lookup_impl",
-        lambda table, index, scale: table.new_empty((index.numel(), table.shape[1])))
-_define("lookup_grad(Tensor grad_out, Tensor index, int rows, float scale, int padding) -> Tensor",
-        "lookup", "_lookup_grad_impl",
-        lambda g, index, rows, scale, padding: g.new_empty((rows, g.shape[1])))
-_define("token_logprobs(Tensor logits, Tensor tokens, float temperature, int ignore_index, "
-        "bool entropy) -> (Tensor, Tensor, Tensor)", "logprobs", "_token_logprobs_impl",
-        lambda z, tokens, temperature, ignore_index, entropy: (
-            _f32(z, z.shape[0]), _f32(z, z.shape[0] if entropy else 0), _f32(z, z.shape[0], 2)))
-_define("token_logprobs_grad(Tensor logits, Tensor tokens, Tensor stats, Tensor entropy, "
-        "Tensor? g, Tensor? g_entropy, float temperature, int ignore_index) -> Tensor",
-        "logprobs", "_token_logprobs_grad_impl",
+# Output shapes of the training operators that launch (the functions above them,
+# embedding_lookup, logprobs, policy, policy_from_logits and preference, are
+# made of these).
+_TRAINING_FAKES = {
+    "lookup": lambda table, index, scale: table.new_empty((index.numel(), table.shape[1])),
+    "lookup_grad": lambda g, index, rows, scale, padding: g.new_empty((rows, g.shape[1])),
+    "token_logprobs": lambda z, tokens, temperature, ignore_index, entropy: (
+        _f32(z, z.shape[0]), _f32(z, z.shape[0] if entropy else 0), _f32(z, z.shape[0], 2)),
+    "token_logprobs_grad":
         lambda z, tokens, stats, entropy, g, g_entropy, temperature, ignore_index:
-        z.new_empty(z.shape))
-_define("policy_loss(Tensor logp, Tensor old_logp, Tensor advantages, Tensor? ref_logp, "
-        "Tensor? mask, Tensor? offsets, bool adv_per_token, float clip_low, float clip_high, "
-        "float kl_coef, int kl, bool sequence_average, bool want_grad) -> (Tensor, Tensor)",
-        "losses", "_policy_loss_impl",
-        lambda logp, *a: (_f32(logp, 4), _f32(logp, logp.shape[0] if a[-1] else 0)))
-_define("scale_tokens(Tensor coef, Tensor values, Tensor g) -> Tensor", "losses",
-        "_scale_tokens_impl", lambda coef, values, g: torch.empty_like(coef))
-_define("policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logp, Tensor advantages, "
-        "Tensor? ref_logp, Tensor? mask, Tensor? offsets, float temperature, bool adv_per_token, "
-        "float clip_low, float clip_high, float kl_coef, int kl, bool sequence_average, "
-        "float grad_scale, bool want_grad) -> (Tensor, Tensor, Tensor)", "losses",
-        "_policy_loss_logits_impl",
-        lambda z, *a: (_f32(z, 4), _f32(z, z.shape[0]),
-                       z.new_empty((z.shape[0] if a[-1] else 0, z.shape[1]))))
-_define("scale_rows_(Tensor(a!) grad, Tensor g, float grad_scale) -> ()", "losses",
-        "_scale_rows_impl", lambda grad, g, grad_scale: None)
-_define("preference_loss(Tensor logp, Tensor offsets, Tensor? ref_logp, Tensor? mask, float beta, "
-        "float smoothing, int kind, bool normalize) -> (Tensor, Tensor, Tensor)", "losses",
-        "_preference_loss_impl",
-        lambda logp, offsets, *a: (_f32(logp), _f32(logp, offsets.shape[0] - 1),
-                                   _f32(logp, offsets.shape[0] - 1)))
-_define("preference_grad(Tensor slope, Tensor offsets, Tensor? mask, Tensor g, int tokens) "
-        "-> Tensor", "losses", "_preference_grad_impl",
-        lambda slope, offsets, mask, g, tokens: _f32(slope, tokens))
+        z.new_empty(z.shape),
+    "policy_loss": lambda logp, *a: (_f32(logp, 4), _f32(logp, logp.shape[0] if a[-1] else 0)),
+    "scale_tokens": lambda coef, values, g: torch.empty_like(coef),
+    "policy_loss_logits": lambda z, *a: (
+        _f32(z, 4), _f32(z, z.shape[0]), z.new_empty((z.shape[0] if a[-1] else 0, z.shape[1]))),
+    "scale_rows_": lambda grad, g, grad_scale: None,
+    "preference_loss": lambda logp, offsets, *a: (
+        _f32(logp), _f32(logp, offsets.shape[0] - 1), _f32(logp, offsets.shape[0] - 1)),
+    "preference_grad": lambda slope, offsets, mask, g, tokens: _f32(slope, tokens),
+}
+
+
+def register_training_fakes() -> None:
+    """Called once, when libsinkslot_b200_torch.so is loaded."""
+    for name, fake in _TRAINING_FAKES.items():
+        torch.library.register_fake(f"{NS}::{name}", fake)
