@@ -6,15 +6,24 @@
 // The gradient's sums run in fp32 in an order that the inputs alone decide (no
 // floating atomics): the tokens are sorted by row (stable, so equal rows keep
 // their order), cut into windows of equal length whatever the rows' counts, and
-// each thread adds up one column vector of one window.  Rows that lie in one window are
-// written at once; rows that cross windows leave partial sums, joined by a
-// second kernel.  Rows that no token names are zeros.
+// each thread adds up one column vector of one window.  Rows that lie in one
+// window are written at once; rows that cross windows leave partial sums, which a
+// second kernel joins.  Rows that no token names are zeros.
+//
+// Memory traffic bounds it: every token's gradient row is read once, the table's
+// gradient is written once (and the rows that are used once more).  Up to 90112
+// tokens are sorted by one cluster through distributed shared memory while the
+// rest of the GPU writes the zeros.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "primitives.h"
 #include "training.h"
 #include "vec.cuh"
 
 namespace sinkslot {
+
+namespace cg = cooperative_groups;
 
 constexpr int kLookThreads = 256;
 
@@ -23,56 +32,111 @@ __device__ __forceinline__ int64_t index_at(const void* index, int bytes, int64_
                     : (int64_t) static_cast<const int32_t*>(index)[t];
 }
 
-// VN elements for each thread: a 16-byte vector, or one element where rows do
-// not begin on such a boundary.
-template <typename T, int VN>
-__global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restrict__ table,
-                                                              int64_t stride, int64_t rows,
-                                                              int64_t dim, int64_t ncv,
-                                                              const void* __restrict__ index,
-                                                              int index_bytes, int64_t count,
-                                                              float scale, T* __restrict__ out) {
-  const int64_t total = count * ncv;
-  for (int64_t q = (int64_t)blockIdx.x * kLookThreads + threadIdx.x; q < total;
-       q += (int64_t)gridDim.x * kLookThreads) {
-    const int64_t t = q / ncv, c = (q - t * ncv) * VN;
-    const int64_t r = index_at(index, index_bytes, t);
-    const bool ok = r >= 0 && r < rows;
-    float f[VN];
-    if constexpr (VN > 1) {
-      if (ok) {
-        unpack(__ldg(reinterpret_cast<const uint4*>(table + r * stride + c)), f, (const T*)nullptr);
-      }
-    } else {
-      if (ok) f[0] = to_f32(table[r * stride + c]);
+// 16 bytes from any element's address, out of the two aligned vectors around it.
+// [begin, end): what may be read.
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p, const T* begin, const T* end) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const uint32_t phase = (uint32_t)(a & 15);
+  const uint4* v = reinterpret_cast<const uint4*>(a - phase);
+  if (phase == 0) return __ldg(v);
+  if (reinterpret_cast<const T*>(v) >= begin && reinterpret_cast<const T*>(v + 2) <= end) {
+    const uint4 lo = __ldg(v), hi = __ldg(v + 1);
+    const uint32_t r = (phase & 3) * 8;
+    uint32_t w0, w1, w2, w3, w4;
+    switch (phase >> 2) {
+      case 0: w0 = lo.x; w1 = lo.y; w2 = lo.z; w3 = lo.w; w4 = hi.x; break;
+      case 1: w0 = lo.y; w1 = lo.z; w2 = lo.w; w3 = hi.x; w4 = hi.y; break;
+      case 2: w0 = lo.z; w1 = lo.w; w2 = hi.x; w3 = hi.y; w4 = hi.z; break;
+      default: w0 = lo.w; w1 = hi.x; w2 = hi.y; w3 = hi.z; w4 = hi.w; break;
     }
+    return make_uint4(__funnelshift_r(w0, w1, r), __funnelshift_r(w1, w2, r),
+                      __funnelshift_r(w2, w3, r), __funnelshift_r(w3, w4, r));
+  }
+  T t[Vec16<T>::N];
 #pragma unroll
-    for (int j = 0; j < VN; ++j) f[j] = ok ? f[j] * scale : __int_as_float(0x7fc00000);
-    if constexpr (VN > 1)
-      *reinterpret_cast<uint4*>(out + t * dim + c) = pack(f, (const T*)nullptr);
-    else
-      out[t * dim + c] = from_f32<T>(f[0]);
+  for (int j = 0; j < Vec16<T>::N; ++j) t[j] = p[j];
+  uint4 u;
+  memcpy(&u, t, 16);
+  return u;
+}
+
+// --------------------------------------------------------------------------
+// Lookup: the output is one array of 16-byte vectors whatever the width of its
+// rows; a vector that two rows share goes element by element.  Four vectors for
+// each thread, so that the index, then the row's data, are waited for once for
+// all four.
+// --------------------------------------------------------------------------
+constexpr int kLookVecs = 4;
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restrict__ table,
+                                                              int64_t stride, int64_t rows, I dim,
+                                                              const void* __restrict__ index,
+                                                              int index_bytes, I total,
+                                                              float scale, T* __restrict__ out) {
+  constexpr int N = Vec16<T>::N;
+  const I vecs = total / N;
+  const T* end = table + (rows - 1) * stride + (int64_t)dim;
+  const I v0 = (I)blockIdx.x * (kLookThreads * kLookVecs) + threadIdx.x;
+  int64_t r[kLookVecs];
+  I c[kLookVecs];
+  uint4 u[kLookVecs];
+#pragma unroll
+  for (int k = 0; k < kLookVecs; ++k) {
+    const I v = v0 + k * kLookThreads;
+    r[k] = -1;
+    c[k] = dim;
+    if (v < vecs) {
+      const I t = v * N / dim;
+      c[k] = v * N - t * dim;
+      r[k] = index_at(index, index_bytes, (int64_t)t);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kLookVecs; ++k)
+    if (c[k] + N <= dim && r[k] >= 0 && r[k] < rows)
+      u[k] = load16(table + r[k] * stride + (int64_t)c[k], table, end);
+#pragma unroll
+  for (int k = 0; k < kLookVecs; ++k) {
+    const I v = v0 + k * kLookThreads;
+    if (v < vecs && c[k] + N <= dim) {
+      float f[N];
+      if (r[k] >= 0 && r[k] < rows) {
+        unpack(u[k], f, (const T*)nullptr);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] *= scale;
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = __int_as_float(0x7fc00000);
+      }
+      reinterpret_cast<uint4*>(out)[v] = pack(f, (const T*)nullptr);
+    } else if (v <= vecs) {
+      for (I e = v * N, stop = v < vecs ? e + N : total; e < stop; ++e) {
+        const I t = e / dim, col = e - t * dim;
+        const int64_t row = index_at(index, index_bytes, (int64_t)t);
+        out[e] = row >= 0 && row < rows
+                     ? from_f32<T>(to_f32(table[row * stride + (int64_t)col]) * scale)
+                     : from_f32<T>(__int_as_float(0x7fc00000));
+      }
+    }
   }
 }
 
-static bool aligned16(const void* p, int64_t stride, int dtype) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * dtype_bytes(dtype) % 16 == 0;
-}
-
 template <typename T>
-static int launch_lookup(const void* table, int dtype, int64_t stride, int64_t rows, int64_t dim,
+static int launch_lookup(const void* table, int64_t stride, int64_t rows, int64_t dim,
                          const void* index, int index_bytes, int64_t count, float scale, void* out,
                          cudaStream_t st) {
-  const bool vec = aligned16(table, stride, dtype) && aligned16(out, dim, dtype);
-  const int64_t ncv = vec ? dim / Vec16<T>::N : dim;
-  int64_t grid = ceil_div64(count * ncv, kLookThreads);
-  if (grid > 0x7fffffff) grid = 0x7fffffff;
-  if (vec)
-    lookup_kernel<T, Vec16<T>::N><<<(unsigned)grid, kLookThreads, 0, st>>>(
-        (const T*)table, stride, rows, dim, ncv, index, index_bytes, count, scale, (T*)out);
+  const int64_t grid = ceil_div64(count * dim / Vec16<T>::N + 1, kLookThreads * kLookVecs);
+  SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup: sizes too large");
+  // (divisions of 64 bits cost as much as the copy: 32 where they do)
+  if (count * dim + kLookThreads * kLookVecs * Vec16<T>::N < (int64_t(1) << 32))
+    lookup_kernel<T, uint32_t><<<(unsigned)grid, kLookThreads, 0, st>>>(
+        (const T*)table, stride, rows, (uint32_t)dim, index, index_bytes, (uint32_t)(count * dim),
+        scale, (T*)out);
   else
-    lookup_kernel<T, 1><<<(unsigned)grid, kLookThreads, 0, st>>>(
-        (const T*)table, stride, rows, dim, ncv, index, index_bytes, count, scale, (T*)out);
+    lookup_kernel<T, int64_t><<<(unsigned)grid, kLookThreads, 0, st>>>(
+        (const T*)table, stride, rows, dim, index, index_bytes, count * dim, scale, (T*)out);
   SINKSLOT_CHECK_LAUNCH();
   return kOk;
 }
@@ -85,150 +149,459 @@ int lookup(const void* table, int dtype, int64_t stride, int64_t rows, int64_t d
   SINKSLOT_REQUIRE(index_bytes == 4 || index_bytes == 8, "lookup: index must be int32 or int64");
   if (count == 0) return kOk;
   SINKSLOT_REQUIRE(table && index && out, "lookup: null argument");
+  SINKSLOT_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0,
+                   "lookup: out must begin on a 16-byte boundary");
   const float s = (float)scale;
   if (dtype == kF32)
-    return launch_lookup<float>(table, dtype, stride, rows, dim, index, index_bytes, count, s, out,
-                                st);
+    return launch_lookup<float>(table, stride, rows, dim, index, index_bytes, count, s, out, st);
   if (dtype == kF16)
-    return launch_lookup<__half>(table, dtype, stride, rows, dim, index, index_bytes, count, s,
-                                 out, st);
-  return launch_lookup<__nv_bfloat16>(table, dtype, stride, rows, dim, index, index_bytes, count,
-                                      s, out, st);
+    return launch_lookup<__half>(table, stride, rows, dim, index, index_bytes, count, s, out, st);
+  return launch_lookup<__nv_bfloat16>(table, stride, rows, dim, index, index_bytes, count, s, out,
+                                      st);
 }
 
 // --------------------------------------------------------------------------
-// Gradient
+// Gradient, first part: the tokens sorted by row.
 // --------------------------------------------------------------------------
-constexpr int kWindow = 32;  // sorted tokens per thread
-constexpr int kAhead = 8;    // loads in flight per thread
 
-// Sort keys: the row, or `rows` for a token that gets no gradient (padding, or
-// an index out of range), which sorts behind all rows.
+// Sort key: the row, or `rows` for a token that gets no gradient (padding, or an
+// index out of range), which sorts behind all rows.
+__device__ __forceinline__ uint32_t key_of(const void* index, int bytes, int64_t t, int64_t rows,
+                                           int64_t padding) {
+  const int64_t r = index_at(index, bytes, t);
+  return (uint32_t)(r < 0 || r >= rows || r == padding ? rows : r);
+}
+
 __global__ void __launch_bounds__(256) lookup_key_kernel(const void* __restrict__ index,
                                                          int index_bytes, int64_t count,
                                                          int64_t rows, int64_t padding,
                                                          uint32_t* __restrict__ keys) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= count) return;
-  const int64_t r = index_at(index, index_bytes, t);
-  keys[t] = (uint32_t)(r < 0 || r >= rows || r == padding ? rows : r);
+  if (t < count) keys[t] = key_of(index, index_bytes, t, rows, padding);
+}
+
+// One cluster (the grid's first) sorts; the other CTAs write the table's zeros.
+// Least significant digit first, 9 bits a pass: the 18 bits of a table of 2^17
+// rows take two.  Each warp ranks a run of its CTA's tokens by digit (match, in
+// order), counts are joined over warps, then over the cluster's CTAs, and every
+// token goes straight to its place in the shared memory of the CTA that holds it
+// in the next pass.
+constexpr int kSortCta = 1024;
+constexpr int kSortCtaWarps = kSortCta / 32;
+constexpr int kDigitBits = 9;
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kSortRounds = 11;  // tokens per thread (their keys and values, twice, fill 227 KB)
+constexpr int kSortMost = 8 * kSortRounds * kSortCta;  // tokens of the largest cluster: 90112
+
+struct SortShared {
+  uint16_t warp_count[kSortCtaWarps][kDigits];
+  uint32_t total[8][kDigits];  // digit counts of the cluster's CTAs
+  uint32_t base[kDigits];      // where this CTA's tokens of a digit begin
+  uint32_t scan[kDigits / 32];
+};
+
+constexpr int64_t kFillWithSort = 32 << 20;  // bytes of zeros that the sort hides
+
+static size_t sort_smem(int per) { return sizeof(SortShared) + (size_t)per * 16; }
+
+__global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
+    const void* __restrict__ index, int index_bytes, int count, int64_t rows, int64_t padding,
+    int per, int bits, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ perm_out,
+    uint32_t* __restrict__ chains, uint4* __restrict__ zeros, int64_t zero_vecs,
+    int64_t zero_tail) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int split = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  chain_release();  // what fills the rest of the table waits for nothing here
+  if ((int)blockIdx.x >= split) {
+    const int64_t at = ((int64_t)blockIdx.x - split) * kSortCta + threadIdx.x;
+    const int64_t step = ((int64_t)gridDim.x - split) * kSortCta;
+    for (int64_t i = at; i < zero_vecs; i += step) zeros[i] = make_uint4(0, 0, 0, 0);
+    if (at < zero_tail) reinterpret_cast<uint16_t*>(zeros + zero_vecs)[at] = 0;
+    return;
+  }
+  extern __shared__ __align__(16) unsigned char raw[];
+  SortShared& sh = *reinterpret_cast<SortShared*>(raw);
+  uint32_t* buf = reinterpret_cast<uint32_t*>(raw + sizeof(SortShared));  // keys, values, twice
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mine = max(0, min(per, count - rank * per));
+  const int run = per / kSortCtaWarps;  // a warp's tokens (per is a multiple of kSortCta)
+  if (rank == 0 && threadIdx.x == 0) chains[0] = 0;
+  int cur = 0;
+  for (int shift = 0; shift < bits; shift += kDigitBits, cur ^= 1) {
+    const bool last = shift + kDigitBits >= bits;
+    for (int i = threadIdx.x; i < kSortCtaWarps * kDigits / 2; i += kSortCta)
+      reinterpret_cast<uint32_t*>(sh.warp_count)[i] = 0;
+    __syncthreads();
+    uint32_t key[kSortRounds], val[kSortRounds];
+    uint16_t loc[kSortRounds];
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (r * 32 >= run) break;
+      const int i = warp * run + r * 32 + lane;
+      const bool on = i < mine;
+      key[r] = val[r] = 0;
+      if (on) {
+        if (shift == 0) {
+          val[r] = (uint32_t)(rank * per + i);
+          key[r] = key_of(index, index_bytes, rank * per + i, rows, padding);
+        } else {
+          key[r] = buf[cur * 2 * per + i];
+          val[r] = buf[cur * 2 * per + per + i];
+        }
+      }
+      const uint32_t dg = on ? (key[r] >> shift) & (kDigits - 1) : kDigits;
+      const uint32_t peers = __match_any_sync(0xffffffffu, dg);
+      const uint32_t before = __popc(peers & ((1u << lane) - 1u));
+      uint32_t base = 0;
+      if (on) base = sh.warp_count[warp][dg];
+      __syncwarp();
+      if (on && before == 0) sh.warp_count[warp][dg] = (uint16_t)(base + __popc(peers));
+      __syncwarp();
+      loc[r] = (uint16_t)(base + before);
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortCtaWarps; ++w) {
+        const uint32_t c = sh.warp_count[w][threadIdx.x];
+        sh.warp_count[w][threadIdx.x] = (uint16_t)sum;
+        sum += c;
+      }
+      for (int k = 0; k < split; ++k)
+        cl.map_shared_rank(&sh.total[0][0], k)[rank * kDigits + threadIdx.x] = sum;
+    }
+    cl.sync();
+    uint32_t all = 0, ahead = 0, incl = 0;
+    if (threadIdx.x < kDigits) {
+      for (int k = 0; k < split; ++k) {
+        const uint32_t c = sh.total[k][threadIdx.x];
+        if (k < rank) ahead += c;
+        all += c;
+      }
+      incl = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      if (lane == 31) sh.scan[warp] = incl;
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      uint32_t before = 0;
+      for (int k = 0; k < warp; ++k) before += sh.scan[k];
+      sh.base[threadIdx.x] = before + incl - all + ahead;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (r * 32 >= run) break;
+      if (warp * run + r * 32 + lane < mine) {
+        const uint32_t dg = (key[r] >> shift) & (kDigits - 1);
+        const uint32_t pos = sh.base[dg] + sh.warp_count[warp][dg] + loc[r];
+        if (last) {
+          keys_out[pos] = key[r];
+          perm_out[pos] = val[r];
+        } else {
+          const uint32_t to = pos / (uint32_t)per, at = pos - to * (uint32_t)per;
+          uint32_t* dst = cl.map_shared_rank(buf, to) + (cur ^ 1) * 2 * per;
+          dst[at] = key[r];
+          dst[per + at] = val[r];
+        }
+      }
+    }
+    // (the last pass as well: no CTA leaves while others read or write its memory)
+    cl.sync();
+  }
+}
+
+// Zeros, 8 KB for each CTA, while the sort runs (launched behind it without
+// waiting for it; the last CTA waits at its end, so that this kernel's completion
+// stands for both).  1 GiB: 7.4 TB/s, where CTAs that stride over the table reach
+// 6.0 and the sort kernel's own spare CTAs 4.4.
+constexpr int kFillVecs = 2;
+__global__ void __launch_bounds__(kLookThreads) lookup_zero_kernel(uint4* __restrict__ zeros,
+                                                                   int64_t vecs, int64_t tail) {
+  const int64_t at = (int64_t)blockIdx.x * (kLookThreads * kFillVecs) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kFillVecs; ++k)
+    if (at + k * kLookThreads < vecs) zeros[at + k * kLookThreads] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x < tail) reinterpret_cast<uint16_t*>(zeros + vecs)[threadIdx.x] = 0;
+    chain_enter();
+  }
+}
+
+// --------------------------------------------------------------------------
+// Gradient, second part: the sums.  VN columns for each thread: a 16-byte vector
+// of the gradient's row, cut by that row's own boundaries (chunk j holds the
+// columns [j VN - shift, (j + 1) VN - shift), shift the row's phase), or, for
+// narrow tables, one column.
+// --------------------------------------------------------------------------
+constexpr int kAhead = 8;  // loads in flight per thread; windows are multiples of it
+
+struct SumArgs {
+  const uint32_t* keys;
+  const uint32_t* perm;
+  int64_t count, rows, stride, dim, ncv;
+  int window;
+  float scale;
+  float* part;
+  uint32_t* chains;  // [0]: how many; then the windows where a crossing row begins
+};
+
+template <typename T, int VN>
+__device__ __forceinline__ int64_t first_column(const T* row, int64_t j) {
+  if (VN == 1) return j;
+  return j * VN - (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
 
 template <typename T, int VN>
-__device__ __forceinline__ void store_row(T* p, const float (&acc)[VN], float scale) {
-  float f[VN];
+__device__ __forceinline__ void store_row(T* row, int64_t j, int64_t dim, const float (&acc)[VN],
+                                          float scale) {
+  const int64_t c = first_column<T, VN>(row, j);
+  if constexpr (VN == 1) {
+    row[c] = from_f32<T>(acc[0] * scale);
+  } else {
+    float f[VN];
 #pragma unroll
-  for (int j = 0; j < VN; ++j) f[j] = acc[j] * scale;
-  if constexpr (VN > 1)
-    *reinterpret_cast<uint4*>(p) = pack(f, (const T*)nullptr);
-  else
-    *p = from_f32<T>(f[0]);
+    for (int k = 0; k < VN; ++k) f[k] = acc[k] * scale;
+    if (c >= 0 && c + VN <= dim) {
+      *reinterpret_cast<uint4*>(row + c) = pack(f, (const T*)nullptr);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VN; ++k)
+        if (c + k >= 0 && c + k < dim) row[c + k] = from_f32<T>(f[k]);
+    }
+  }
+}
+
+template <int VN>
+__device__ __forceinline__ float* part_at(const SumArgs& a, int64_t slot, int64_t j) {
+  return a.part + (slot * a.ncv + j) * VN;
 }
 
 template <int VN>
 __device__ __forceinline__ void store_part(float* p, const float (&acc)[VN]) {
 #pragma unroll
-  for (int j = 0; j < VN; ++j) p[j] = acc[j];
+  for (int k = 0; k < VN; ++k) p[k] = acc[k];
 }
 
-// part[(2 w + 0) dim ...]: the sum of window w's first row where that row began
-// in an earlier window; part[(2 w + 1) dim ...]: of its last row where it began
-// here and goes on in the next window.
+// Where a finished sum goes.  part slot 2 w: the sum of window w's first row where
+// that row began in an earlier window; 2 w + 1: of its last row where it began here
+// and goes on.  (Not inlined: the summing loops call it at each of their steps.)
 template <typename T, int VN>
-__global__ void __launch_bounds__(kLookThreads) lookup_grad_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ perm, int64_t count,
-    int64_t rows, const T* __restrict__ g, int64_t stride, int64_t dim, int64_t ncv, float scale,
-    T* __restrict__ out, float* __restrict__ part) {
-  const int64_t q = (int64_t)blockIdx.x * kLookThreads + threadIdx.x;
-  const int64_t w = q / ncv, c = (q - w * ncv) * VN;
-  const int64_t i0 = w * kWindow;
-  if (i0 >= count) return;
-  const int n = (int)min((int64_t)kWindow, count - i0);
-  uint32_t cur = keys[i0];
-  if (cur >= rows) return;
-  bool head = i0 > 0 && keys[i0 - 1] == cur;
+__device__ __noinline__ void put_row(T* out, int64_t dim, uint32_t row, int64_t j, float scale,
+                                     float a0, float a1, float a2, float a3, float a4, float a5,
+                                     float a6, float a7) {
+  const float all[8] = {a0, a1, a2, a3, a4, a5, a6, a7};
   float acc[VN];
 #pragma unroll
-  for (int j = 0; j < VN; ++j) acc[j] = 0.0f;
+  for (int k = 0; k < VN; ++k) acc[k] = all[k];
+  store_row<T, VN>(out + (int64_t)row * dim, j, dim, acc, scale);
+}
+
+template <typename T, int VN>
+__device__ __forceinline__ void put_sum(const SumArgs& a, T* out, bool head, int64_t w, int64_t j,
+                                        uint32_t row, const float (&acc)[VN]) {
+  if (head) {
+    store_part<VN>(part_at<VN>(a, 2 * w, j), acc);
+  } else if constexpr (VN == 8) {
+    put_row<T, VN>(out, a.dim, row, j, a.scale, acc[0], acc[1], acc[2], acc[3], acc[4], acc[5],
+                   acc[6], acc[7]);
+  } else if constexpr (VN == 4) {
+    put_row<T, VN>(out, a.dim, row, j, a.scale, acc[0], acc[1], acc[2], acc[3], 0, 0, 0, 0);
+  } else {
+    store_row<T, VN>(out + (int64_t)row * a.dim, j, a.dim, acc, a.scale);
+  }
+}
+
+// kAligned: all rows of both arrays begin on 16-byte boundaries.  The windows'
+// keys and positions are staged in shared memory where a CTA meets few windows
+// (ncv of kStageFrom or more).
+constexpr int kStageFrom = 64;
+constexpr int kStaged = (kLookThreads / kStageFrom + 1) * 64;
+
+template <typename T, int VN, bool kAligned, bool kStage>
+__global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
+                                                                  const T* __restrict__ g,
+                                                                  T* __restrict__ out) {
+  __shared__ uint2 staged[kStage ? kStaged : 1];
+  const int64_t q = (int64_t)blockIdx.x * kLookThreads + threadIdx.x;
+  const int64_t w = q / a.ncv, j = q - w * a.ncv;
+  const int64_t i0 = w * a.window;
+  int64_t s0 = 0;
+  if constexpr (kStage) {
+    s0 = (int64_t)blockIdx.x * kLookThreads / a.ncv * a.window;
+    const int64_t s1 =
+        min(a.count, (((int64_t)blockIdx.x + 1) * kLookThreads - 1) / a.ncv * a.window + a.window);
+    for (int64_t i = s0 + threadIdx.x; i < s1; i += kLookThreads)
+      staged[i - s0] = make_uint2(a.keys[i], a.perm[i]);
+    __syncthreads();
+  }
+  auto entry = [&](int64_t i) {
+    if constexpr (kStage)
+      return staged[i - s0];
+    else
+      return make_uint2(a.keys[i], a.perm[i]);
+  };
+  chain_release();
+  if (i0 >= a.count) return;
+  const int n = (int)min((int64_t)a.window, a.count - i0);
+  uint32_t cur = entry(i0).x;
+  if (cur >= a.rows) return;
+  const T* gend = g + (a.count - 1) * a.stride + a.dim;
+  bool head = i0 > 0 && a.keys[i0 - 1] == cur;
+  float acc[VN];
+#pragma unroll
+  for (int k = 0; k < VN; ++k) acc[k] = 0.0f;
   for (int b = 0; b < n; b += kAhead) {
     uint32_t key[kAhead];
-    float f[kAhead][VN];
+    uint4 u[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      key[k] = b + k < n ? keys[i0 + b + k] : 0xffffffffu;
-      if (key[k] < rows) {
-        const T* p = g + (int64_t)perm[i0 + b + k] * stride + c;
-        if constexpr (VN > 1)
-          unpack(__ldg(reinterpret_cast<const uint4*>(p)), f[k], (const T*)nullptr);
-        else
-          f[k][0] = to_f32(*p);
+      const uint2 en = b + k < n ? entry(i0 + b + k) : make_uint2(0xffffffffu, 0);
+      key[k] = en.x;
+      u[k] = make_uint4(0, 0, 0, 0);
+      if (key[k] < a.rows) {
+        const T* p = g + (int64_t)en.y * a.stride;
+        if constexpr (VN == 1) {
+          u[k].x = __float_as_uint(to_f32(p[j]));
+        } else if constexpr (kAligned) {
+          u[k] = __ldg(reinterpret_cast<const uint4*>(p) + j);
+        } else {
+          const int64_t c = first_column<T, VN>(out + (int64_t)key[k] * a.dim, j);
+          if (c >= 0 && c + VN <= a.dim) {
+            u[k] = load16(p + c, g, gend);
+          } else {
+            T t[VN];
+#pragma unroll
+            for (int m = 0; m < VN; ++m)
+              t[m] = c + m >= 0 && c + m < a.dim ? p[c + m] : from_f32<T>(0.0f);
+            memcpy(&u[k], t, 16);
+          }
+        }
       }
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (b + k >= n) break;
       if (key[k] != cur) {
-        if (head)
-          store_part<VN>(part + 2 * w * dim + c, acc);
-        else
-          store_row<T, VN>(out + (int64_t)cur * dim + c, acc, scale);
+        put_sum<T, VN>(a, out, head, w, j, cur, acc);
         head = false;
         cur = key[k];
-        if (cur >= rows) return;  // the tokens without a gradient
+        if (cur >= a.rows) return;  // the tokens without a gradient
 #pragma unroll
-        for (int j = 0; j < VN; ++j) acc[j] = 0.0f;
+        for (int m = 0; m < VN; ++m) acc[m] = 0.0f;
       }
+      if constexpr (VN == 1) {
+        acc[0] += __uint_as_float(u[k].x);
+      } else {
+        float f[VN];
+        unpack(u[k], f, (const T*)nullptr);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) acc[j] += f[k][j];
+        for (int m = 0; m < VN; ++m) acc[m] += f[m];
+      }
     }
   }
-  const bool on = i0 + n < count && keys[i0 + n] == cur;
-  if (head)
-    store_part<VN>(part + 2 * w * dim + c, acc);
-  else if (on)
-    store_part<VN>(part + (2 * w + 1) * dim + c, acc);
-  else
-    store_row<T, VN>(out + (int64_t)cur * dim + c, acc, scale);
+  if (!head && i0 + n < a.count && a.keys[i0 + n] == cur) {
+    store_part<VN>(part_at<VN>(a, 2 * w + 1, j), acc);
+    // (the order of the list decides nothing but who joins which row)
+    if (j == 0) a.chains[1 + atomicAdd(a.chains, 1u)] = (uint32_t)w;
+  } else {
+    put_sum<T, VN>(a, out, head, w, j, cur, acc);
+  }
 }
 
-// Rows that begin in window w and go on behind it.
+// Rows that cross windows: 32 chunks of columns for each CTA, its warps share the
+// row's windows in order and their sums are joined in order.
 template <typename T, int VN>
-__global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(
-    const uint32_t* __restrict__ keys, int64_t count, int64_t rows, int64_t dim, int64_t ncv,
-    float scale, const float* __restrict__ part, T* __restrict__ out) {
-  const int64_t q = (int64_t)blockIdx.x * kLookThreads + threadIdx.x;
-  const int64_t w = q / ncv, c = (q - w * ncv) * VN;
-  const int64_t i0 = w * kWindow, i1 = i0 + kWindow;
-  if (i1 >= count) return;
-  const uint32_t cur = keys[i1 - 1];
-  if (cur >= rows || keys[i1] != cur) return;
-  if (i0 > 0 && keys[i0] == cur && keys[i0 - 1] == cur) return;  // began earlier
-  float acc[VN];
-  const float* p = part + (2 * w + 1) * dim + c;
+__global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a,
+                                                                   T* __restrict__ out) {
+  constexpr int kWarps = kLookThreads / 32;
+  __shared__ float sums[kWarps][32][VN + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.y * 32 + lane;
+  chain_enter();
+  const uint32_t chains = a.chains[0];
+  const int64_t windows = (a.count + a.window - 1) / a.window;
+  for (uint32_t item = blockIdx.x; item < chains; item += gridDim.x) {
+    const int64_t w = a.chains[1 + item];
+    const uint32_t cur = a.keys[(w + 1) * a.window - 1];
+    // the first window after w that does not begin with this row: 32 probes a step
+    int64_t lo = w + 1, hi = windows;  // lo begins with it; the answer is in (lo, hi]
+    while (hi - lo > 1) {
+      const int64_t step = (hi - lo + 31) / 32;
+      const int64_t at = lo + step * (lane + 1);
+      const bool same = at < hi && a.keys[at * a.window] == cur;
+      const int found = __popc(__ballot_sync(0xffffffffu, same));  // a prefix of the lanes
+      const int64_t next = lo + step * (found + 1);
+      lo += step * found;
+      if (next < hi) hi = next;
+    }
+    const int64_t n = hi - w;  // partial sums: w's tail, the heads of the windows behind
+    const int64_t k0 = n * warp / kWarps, k1 = n * (warp + 1) / kWarps;
+    float acc[VN];
 #pragma unroll
-  for (int j = 0; j < VN; ++j) acc[j] = p[j];
-  for (int64_t k = w + 1; k * kWindow < count && keys[k * kWindow] == cur; ++k) {
-    p = part + 2 * k * dim + c;
+    for (int m = 0; m < VN; ++m) acc[m] = 0.0f;
+    if (j < a.ncv) {
+#pragma unroll 4
+      for (int64_t k = k0; k < k1; ++k) {
+        const float* p = part_at<VN>(a, 2 * (w + k) + (k == 0), j);
+        if constexpr (VN == 1) {
+          acc[0] += *p;
+        } else {
 #pragma unroll
-    for (int j = 0; j < VN; ++j) acc[j] += p[j];
+          for (int m = 0; m < VN; m += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + m);
+            acc[m] += v.x; acc[m + 1] += v.y; acc[m + 2] += v.z; acc[m + 3] += v.w;
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < VN; ++m) sums[warp][lane][m] = acc[m];
+    __syncthreads();
+    if (warp == 0 && j < a.ncv) {
+      for (int k = 1; k < kWarps; ++k) {
+#pragma unroll
+        for (int m = 0; m < VN; ++m) acc[m] += sums[k][lane][m];
+      }
+      store_row<T, VN>(out + (int64_t)cur * a.dim, j, a.dim, acc, a.scale);
+    }
   }
-  store_row<T, VN>(out + (int64_t)cur * dim + c, acc, scale);
+}
+
+// Tokens per window: as few as keep the GPU's threads busy about once over (small
+// calls want threads, large ones few partial sums), at most 64.
+static int window_of(int64_t count, int64_t dim) {
+  int w = kAhead;
+  while (w < 64 && count / w * (dim / 8 + 1) > (int64_t)kNumSMs * 1024) w *= 2;
+  return w;
 }
 
 struct LookWs {
-  uint32_t *k1, *v1, *k2, *v2;
+  uint32_t *k1, *v1, *k2, *v2, *chains;
   int64_t *hist, *stmp;
   float* part;
 };
 
 static void carve_look(Carver& cv, LookWs& w, int64_t count, int64_t dim) {
   const int64_t e = count > 0 ? count : 1;
+  const int64_t windows = ceil_div64(e, window_of(e, dim));
+  w.chains = cv.take<uint32_t>(windows + 1);
   w.k1 = cv.take<uint32_t>(e); w.v1 = cv.take<uint32_t>(e);
-  w.k2 = cv.take<uint32_t>(e); w.v2 = cv.take<uint32_t>(e);
-  const int64_t nh = radix_hist_elems(1, e);
-  w.hist = cv.take<int64_t>(nh);
-  w.stmp = cv.take<int64_t>(scan_tmp_elems(nh));
-  w.part = cv.take<float>((size_t)(2 * ceil_div64(e, kWindow) * dim));
+  w.k2 = w.v2 = nullptr;
+  w.hist = w.stmp = nullptr;
+  if (e > kSortMost) {
+    w.k2 = cv.take<uint32_t>(e); w.v2 = cv.take<uint32_t>(e);
+    const int64_t nh = radix_hist_elems(1, e);
+    w.hist = cv.take<int64_t>(nh);
+    w.stmp = cv.take<int64_t>(scan_tmp_elems(nh));
+  }
+  w.part = cv.take<float>((size_t)(2 * windows * (dim + 16)));  // a row cut by its boundaries
 }
 
 size_t lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t dim) {
@@ -239,19 +612,99 @@ size_t lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t dim) {
   return cv.used;
 }
 
-template <typename T, int VN>
-static int launch_sums(const uint32_t* keys, const uint32_t* perm, int64_t count, int64_t rows,
-                       const void* g, int64_t stride, int64_t dim, float scale, void* out,
-                       float* part, cudaStream_t st) {
-  const int64_t ncv = dim / VN;
-  const int64_t grid = ceil_div64(ceil_div64(count, kWindow) * ncv, kLookThreads);
-  SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup_grad: sizes too large");
-  lookup_grad_kernel<T, VN><<<(unsigned)grid, kLookThreads, 0, st>>>(
-      keys, perm, count, rows, (const T*)g, stride, dim, ncv, scale, (T*)out, part);
+template <typename T, int VN, bool kAligned>
+static int launch_sums(SumArgs a, const void* g, void* out, cudaStream_t st) {
+  a.ncv = kAligned ? a.dim / VN : (a.dim + 2 * VN - 2) / VN;
+  const int64_t windows = ceil_div64(a.count, a.window);
+  const int64_t grid = ceil_div64(windows * a.ncv, kLookThreads);
+  const int64_t groups = ceil_div64(a.ncv, 32);
+  SINKSLOT_REQUIRE(grid <= 0x7fffffff && groups <= 65535, "lookup_grad: sizes too large");
+  if (a.ncv >= kStageFrom)
+    lookup_sum_kernel<T, VN, kAligned, true><<<(unsigned)grid, kLookThreads, 0, st>>>(
+        a, (const T*)g, (T*)out);
+  else
+    lookup_sum_kernel<T, VN, kAligned, false><<<(unsigned)grid, kLookThreads, 0, st>>>(
+        a, (const T*)g, (T*)out);
   SINKSLOT_CHECK_LAUNCH();
-  lookup_join_kernel<T, VN><<<(unsigned)grid, kLookThreads, 0, st>>>(
-      keys, count, rows, dim, ncv, scale, part, (T*)out);
-  SINKSLOT_CHECK_LAUNCH();
+  if (windows == 1) return kOk;  // nothing crosses
+  int64_t x = ceil_div64(6 * num_sms(), groups);
+  if (x > windows) x = windows;
+  SINKSLOT_CUDA_TRY(launch_chained(lookup_join_kernel<T, VN>, dim3((unsigned)x, (unsigned)groups),
+                                   dim3(kLookThreads), 0, st, a, (T*)out));
+  return kOk;
+}
+
+template <typename T>
+static int launch_sums_of(SumArgs a, const void* g, void* out, cudaStream_t st) {
+  constexpr int N = Vec16<T>::N;
+  // under two vectors, a thread for each column: vectors would be mostly edges
+  if (a.dim < 2 * N) return launch_sums<T, 1, true>(a, g, out, st);
+  const bool rows16 = (reinterpret_cast<uintptr_t>(g) & 15) == 0 && a.dim % N == 0 &&
+                      a.stride % N == 0;
+  return rows16 ? launch_sums<T, N, true>(a, g, out, st) : launch_sums<T, N, false>(a, g, out, st);
+}
+
+// Sorts the tokens and writes the table's zeros.
+static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_t rows,
+                       int64_t padding, void* out, int64_t out_bytes, LookWs& w,
+                       const uint32_t** keys, const uint32_t** perm, cudaStream_t st) {
+  const int bits = bits_for((uint64_t)rows + 1);
+  if (count > kSortMost) {
+    SINKSLOT_CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)out_bytes, st));
+    SINKSLOT_CUDA_TRY(cudaMemsetAsync(w.chains, 0, sizeof(uint32_t), st));
+    lookup_key_kernel<<<(unsigned)ceil_div64(count, 256), 256, 0, st>>>(index, index_bytes, count,
+                                                                       rows, padding, w.k1);
+    SINKSLOT_CHECK_LAUNCH();
+    bool alt = false;
+    SINKSLOT_TRY(radix_sort_pairs<uint32_t>(w.k1, w.v1, w.k2, w.v2, true, 1, count, bits, w.hist,
+                                            w.stmp, &alt, st));
+    *keys = alt ? w.k2 : w.k1;
+    *perm = alt ? w.v2 : w.v1;
+    return kOk;
+  }
+  int split = 1;
+  while (split < 8 && count > (int64_t)split * 4 * kSortCta) split *= 2;
+  const int per = (int)(ceil_div64(ceil_div64(count, split), kSortCta) * kSortCta);
+  {
+    // the shared-memory limit is a per-device function attribute
+    static bool configured[64] = {};
+    int dev = 0;
+    SINKSLOT_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+      SINKSLOT_CUDA_TRY(cudaFuncSetAttribute(lookup_sort_kernel,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)sort_smem(kSortRounds * kSortCta)));
+      if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+  }
+  // zeros: by spare CTAs of the sort's own launch while that hides them
+  const int64_t vecs = out_bytes / 16, tail = (out_bytes - vecs * 16) / 2;
+  const bool apart = out_bytes > kFillWithSort;
+  int64_t fill = apart ? 0 : ceil_div64(vecs > 0 ? vecs : 1, (int64_t)kSortCta * 4);
+  const int64_t room = num_sms() - split;
+  if (fill > room) fill = room;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(split + ceil_div64(fill, split) * split));
+  cfg.blockDim = dim3(kSortCta);
+  cfg.dynamicSmemBytes = sort_smem(per);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SINKSLOT_CUDA_TRY(cudaLaunchKernelEx(
+      &cfg, lookup_sort_kernel, index, index_bytes, (int)count, rows, padding, per, bits, w.k1,
+      w.v1, w.chains, (uint4*)out, vecs, tail));
+  if (apart) {
+    const int64_t grid = ceil_div64(vecs, kLookThreads * kFillVecs);
+    SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup_grad: sizes too large");
+    SINKSLOT_CUDA_TRY(launch_chained(lookup_zero_kernel, dim3((unsigned)grid), dim3(kLookThreads),
+                                     0, st, (uint4*)out, vecs, tail));
+  }
+  *keys = w.k1;
+  *perm = w.v1;
   return kOk;
 }
 
@@ -265,8 +718,13 @@ int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* ind
   SINKSLOT_REQUIRE(index_bytes == 4 || index_bytes == 8,
                    "lookup_grad: index must be int32 or int64");
   SINKSLOT_REQUIRE(grad_table, "lookup_grad: null argument");
-  SINKSLOT_CUDA_TRY(cudaMemsetAsync(grad_table, 0, (size_t)(rows * dim) * dtype_bytes(dtype), st));
-  if (count == 0) return kOk;
+  SINKSLOT_REQUIRE((reinterpret_cast<uintptr_t>(grad_table) & 15) == 0,
+                   "lookup_grad: grad_table must begin on a 16-byte boundary");
+  const int64_t out_bytes = rows * dim * dtype_bytes(dtype);
+  if (count == 0) {
+    SINKSLOT_CUDA_TRY(cudaMemsetAsync(grad_table, 0, (size_t)out_bytes, st));
+    return kOk;
+  }
   SINKSLOT_REQUIRE(grad_out && index && ws, "lookup_grad: null argument");
   Carver cv(ws, ws_bytes);
   LookWs w;
@@ -275,25 +733,20 @@ int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* ind
     set_error("lookup_grad: workspace too small");
     return kWorkspaceTooSmall;
   }
-  lookup_key_kernel<<<(unsigned)ceil_div64(count, 256), 256, 0, st>>>(index, index_bytes, count,
-                                                                     rows, padding, w.k1);
-  SINKSLOT_CHECK_LAUNCH();
-  bool alt = false;
-  SINKSLOT_TRY(radix_sort_pairs<uint32_t>(w.k1, w.v1, w.k2, w.v2, true, 1, count,
-                                          bits_for((uint64_t)rows + 1), w.hist, w.stmp, &alt, st));
-  const uint32_t* keys = alt ? w.k2 : w.k1;
-  const uint32_t* perm = alt ? w.v2 : w.v1;
-  const float s = (float)scale;
-  const bool vec = aligned16(grad_out, stride, dtype) && aligned16(grad_table, dim, dtype);
-#define GO(T)                                                                                    \
-  return vec ? launch_sums<T, Vec16<T>::N>(keys, perm, count, rows, grad_out, stride, dim, s,    \
-                                           grad_table, w.part, st)                               \
-             : launch_sums<T, 1>(keys, perm, count, rows, grad_out, stride, dim, s, grad_table,  \
-                                 w.part, st)
-  if (dtype == kF32) GO(float);
-  if (dtype == kF16) GO(__half);
-  GO(__nv_bfloat16);
-#undef GO
+  SumArgs a = {};
+  SINKSLOT_TRY(sort_tokens(index, index_bytes, count, rows, padding, grad_table, out_bytes, w,
+                           &a.keys, &a.perm, st));
+  a.count = count;
+  a.rows = rows;
+  a.stride = stride;
+  a.dim = dim;
+  a.window = window_of(count, dim);
+  a.scale = (float)scale;
+  a.part = w.part;
+  a.chains = w.chains;
+  if (dtype == kF32) return launch_sums_of<float>(a, grad_out, grad_table, st);
+  if (dtype == kF16) return launch_sums_of<__half>(a, grad_out, grad_table, st);
+  return launch_sums_of<__nv_bfloat16>(a, grad_out, grad_table, st);
 }
 
 }  // namespace sinkslot

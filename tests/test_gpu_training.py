@@ -250,7 +250,8 @@ def _check_lookup(sk, table, index, scale, padding=None):
 @pytest.mark.parametrize("rows,dim,tokens", [(1, 1, 1), (3, 3, 50), (256, 3, 10000), (7, 16, 31),
                                              (5, 8, 32), (1000, 64, 33), (50, 771, 4097),
                                              (9000, 1032, 700), (2, 257, 20000), (70000, 24, 5000),
-                                             (300, 4100, 64)])
+                                             (300, 4100, 64), (150000, 5, 90112),
+                                             (600, 9, 90113), (1 << 20, 2, 200001), (40, 40, 65000)])
 def test_lookup_sizes(sk, rows, dim, tokens, dtype):
     gen = _gen(rows + dim + tokens)
     table = torch.randn(rows, dim, generator=gen, device="cuda").to(dtype)
@@ -262,7 +263,7 @@ def test_lookup_sizes(sk, rows, dim, tokens, dtype):
 def test_lookup_one_hot_row_and_runs_at_window_ends(sk):
     gen = _gen(5)
     table = torch.randn(40, 20, generator=gen, device="cuda")
-    for n in (31, 32, 33, 64, 65, 96, 1000):
+    for n in (7, 8, 9, 16, 31, 32, 33, 64, 65, 96, 1000, 70000):
         _check_lookup(sk, table.clone(), torch.full((n,), 39, device="cuda"), 2.0)
         mixed = torch.zeros(n, dtype=torch.int64, device="cuda")
         mixed[n // 2:] = 7
