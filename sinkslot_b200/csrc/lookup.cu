@@ -33,29 +33,33 @@ __device__ __forceinline__ int64_t index_at(const void* index, int bytes, int64_
 }
 
 // 16 bytes from any element's address, out of the two aligned vectors around it.
-// [begin, end): what may be read.
+// [begin, end): what may be read; elements outside come as zeros (callers ask for
+// vectors that reach over a row's ends, and drop what is not the row's).
 template <typename T>
 __device__ __forceinline__ uint4 load16(const T* p, const T* begin, const T* end) {
+  constexpr int N = Vec16<T>::N;
   const uintptr_t a = reinterpret_cast<uintptr_t>(p);
   const uint32_t phase = (uint32_t)(a & 15);
-  const uint4* v = reinterpret_cast<const uint4*>(a - phase);
-  if (phase == 0) return __ldg(v);
-  if (reinterpret_cast<const T*>(v) >= begin && reinterpret_cast<const T*>(v + 2) <= end) {
-    const uint4 lo = __ldg(v), hi = __ldg(v + 1);
+  const T* v = reinterpret_cast<const T*>(a - phase);
+  if (v >= begin && v + 2 * N <= end) {
+    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(v));
+    if (phase == 0) return lo;
+    const uint4 hi = __ldg(reinterpret_cast<const uint4*>(v) + 1);
+    // shifted by two words, by one, then by the bytes within a word (selects: the
+    // phase is another for every row)
+    const bool two = phase & 8, one = phase & 4;
+    const uint32_t x0 = two ? lo.z : lo.x, x1 = two ? lo.w : lo.y, x2 = two ? hi.x : lo.z,
+                   x3 = two ? hi.y : lo.w, x4 = two ? hi.z : hi.x, x5 = two ? hi.w : hi.y;
+    const uint32_t y0 = one ? x1 : x0, y1 = one ? x2 : x1, y2 = one ? x3 : x2,
+                   y3 = one ? x4 : x3, y4 = one ? x5 : x4;
+    if (sizeof(T) == 4) return make_uint4(y0, y1, y2, y3);
     const uint32_t r = (phase & 3) * 8;
-    uint32_t w0, w1, w2, w3, w4;
-    switch (phase >> 2) {
-      case 0: w0 = lo.x; w1 = lo.y; w2 = lo.z; w3 = lo.w; w4 = hi.x; break;
-      case 1: w0 = lo.y; w1 = lo.z; w2 = lo.w; w3 = hi.x; w4 = hi.y; break;
-      case 2: w0 = lo.z; w1 = lo.w; w2 = hi.x; w3 = hi.y; w4 = hi.z; break;
-      default: w0 = lo.w; w1 = hi.x; w2 = hi.y; w3 = hi.z; w4 = hi.w; break;
-    }
-    return make_uint4(__funnelshift_r(w0, w1, r), __funnelshift_r(w1, w2, r),
-                      __funnelshift_r(w2, w3, r), __funnelshift_r(w3, w4, r));
+    return make_uint4(__funnelshift_r(y0, y1, r), __funnelshift_r(y1, y2, r),
+                      __funnelshift_r(y2, y3, r), __funnelshift_r(y3, y4, r));
   }
-  T t[Vec16<T>::N];
+  T t[N];
 #pragma unroll
-  for (int j = 0; j < Vec16<T>::N; ++j) t[j] = p[j];
+  for (int j = 0; j < N; ++j) t[j] = p + j >= begin && p + j < end ? p[j] : from_f32<T>(0.0f);
   uint4 u;
   memcpy(&u, t, 16);
   return u;
@@ -63,13 +67,15 @@ __device__ __forceinline__ uint4 load16(const T* p, const T* begin, const T* end
 
 // --------------------------------------------------------------------------
 // Lookup: the output is one array of 16-byte vectors whatever the width of its
-// rows; a vector that two rows share goes element by element.  Four vectors for
-// each thread, so that the index, then the row's data, are waited for once for
-// all four.
+// rows, so a vector may hold the end of one row and the beginning of the next.
+// Four vectors for each thread: the index, then the rows' data, are waited for
+// once for all four.
 // --------------------------------------------------------------------------
 constexpr int kLookVecs = 4;
 
-template <typename T, typename I>
+// kAligned: all rows begin on 16-byte boundaries.  I: 32 bits where the output's
+// elements fit (a division of 64 bits costs more than the copy).
+template <typename T, typename I, bool kAligned>
 __global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restrict__ table,
                                                               int64_t stride, int64_t rows, I dim,
                                                               const void* __restrict__ index,
@@ -79,64 +85,104 @@ __global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restric
   const I vecs = total / N;
   const T* end = table + (rows - 1) * stride + (int64_t)dim;
   const I v0 = (I)blockIdx.x * (kLookThreads * kLookVecs) + threadIdx.x;
-  int64_t r[kLookVecs];
+  int64_t r[kLookVecs], next[kLookVecs];
   I c[kLookVecs];
-  uint4 u[kLookVecs];
+  uint4 u[kLookVecs], w[kLookVecs];
 #pragma unroll
   for (int k = 0; k < kLookVecs; ++k) {
     const I v = v0 + k * kLookThreads;
-    r[k] = -1;
-    c[k] = dim;
+    r[k] = next[k] = -1;
+    c[k] = 0;
     if (v < vecs) {
       const I t = v * N / dim;
       c[k] = v * N - t * dim;
       r[k] = index_at(index, index_bytes, (int64_t)t);
+      if (!kAligned && c[k] + N > dim) next[k] = index_at(index, index_bytes, (int64_t)t + 1);
     }
   }
 #pragma unroll
-  for (int k = 0; k < kLookVecs; ++k)
-    if (c[k] + N <= dim && r[k] >= 0 && r[k] < rows)
-      u[k] = load16(table + r[k] * stride + (int64_t)c[k], table, end);
+  for (int k = 0; k < kLookVecs; ++k) {
+    if (r[k] >= 0 && r[k] < rows) {
+      const T* p = table + r[k] * stride + (int64_t)c[k];
+      u[k] = kAligned ? __ldg(reinterpret_cast<const uint4*>(p)) : load16(p, table, end);
+    }
+    if (!kAligned && next[k] >= 0 && next[k] < rows)
+      w[k] = load16(table + next[k] * stride + (int64_t)c[k] - (int64_t)dim, table, end);
+  }
 #pragma unroll
   for (int k = 0; k < kLookVecs; ++k) {
     const I v = v0 + k * kLookThreads;
-    if (v < vecs && c[k] + N <= dim) {
-      float f[N];
-      if (r[k] >= 0 && r[k] < rows) {
-        unpack(u[k], f, (const T*)nullptr);
+    if (v >= vecs) continue;
+    float f[N];
+    if (r[k] >= 0 && r[k] < rows) {
+      unpack(u[k], f, (const T*)nullptr);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] *= scale;
-      } else {
+      for (int j = 0; j < N; ++j) f[j] *= scale;
+    } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = __int_as_float(0x7fc00000);
-      }
-      reinterpret_cast<uint4*>(out)[v] = pack(f, (const T*)nullptr);
-    } else if (v <= vecs) {
-      for (I e = v * N, stop = v < vecs ? e + N : total; e < stop; ++e) {
-        const I t = e / dim, col = e - t * dim;
-        const int64_t row = index_at(index, index_bytes, (int64_t)t);
-        out[e] = row >= 0 && row < rows
-                     ? from_f32<T>(to_f32(table[row * stride + (int64_t)col]) * scale)
-                     : from_f32<T>(__int_as_float(0x7fc00000));
-      }
+      for (int j = 0; j < N; ++j) f[j] = __int_as_float(0x7fc00000);
     }
+    if (!kAligned && c[k] + N > dim) {
+      float h[N];
+      const bool on = next[k] >= 0 && next[k] < rows;
+      if (on) unpack(w[k], h, (const T*)nullptr);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c[k] + j >= dim) f[j] = on ? h[j] * scale : __int_as_float(0x7fc00000);
+    }
+    reinterpret_cast<uint4*>(out)[v] = pack(f, (const T*)nullptr);
   }
+  if (!kAligned && blockIdx.x == 0 && threadIdx.x < total - vecs * N) {
+    const I e = vecs * N + threadIdx.x, t = e / dim;
+    const int64_t row = index_at(index, index_bytes, (int64_t)t);
+    out[e] = from_f32<T>(row >= 0 && row < rows
+                             ? to_f32(table[row * stride + (int64_t)(e - t * dim)]) * scale
+                             : __int_as_float(0x7fc00000));
+  }
+}
+
+// Rows narrower than a vector: an element for each thread.
+template <typename T>
+__global__ void __launch_bounds__(kLookThreads) lookup_narrow_kernel(
+    const T* __restrict__ table, int64_t stride, int64_t rows, uint32_t dim,
+    const void* __restrict__ index, int index_bytes, int64_t total, float scale,
+    T* __restrict__ out) {
+  const int64_t e = (int64_t)blockIdx.x * kLookThreads + threadIdx.x;
+  if (e >= total) return;
+  const int64_t t = total < (int64_t(1) << 32) ? (int64_t)((uint32_t)e / dim) : e / dim;
+  const int64_t row = index_at(index, index_bytes, t);
+  out[e] = from_f32<T>(row >= 0 && row < rows ? to_f32(table[row * stride + (e - t * dim)]) * scale
+                                              : __int_as_float(0x7fc00000));
 }
 
 template <typename T>
 static int launch_lookup(const void* table, int64_t stride, int64_t rows, int64_t dim,
                          const void* index, int index_bytes, int64_t count, float scale, void* out,
                          cudaStream_t st) {
-  const int64_t grid = ceil_div64(count * dim / Vec16<T>::N + 1, kLookThreads * kLookVecs);
+  constexpr int N = Vec16<T>::N;
+  const int64_t total = count * dim;
+  if (dim < N) {
+    const int64_t grid = ceil_div64(total, kLookThreads);
+    SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup: sizes too large");
+    lookup_narrow_kernel<T><<<(unsigned)grid, kLookThreads, 0, st>>>(
+        (const T*)table, stride, rows, (uint32_t)dim, index, index_bytes, total, scale, (T*)out);
+    SINKSLOT_CHECK_LAUNCH();
+    return kOk;
+  }
+  const int64_t grid = ceil_div64(total / N + 1, kLookThreads * kLookVecs);
   SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup: sizes too large");
-  // (divisions of 64 bits cost as much as the copy: 32 where they do)
-  if (count * dim + kLookThreads * kLookVecs * Vec16<T>::N < (int64_t(1) << 32))
-    lookup_kernel<T, uint32_t><<<(unsigned)grid, kLookThreads, 0, st>>>(
-        (const T*)table, stride, rows, (uint32_t)dim, index, index_bytes, (uint32_t)(count * dim),
-        scale, (T*)out);
-  else
-    lookup_kernel<T, int64_t><<<(unsigned)grid, kLookThreads, 0, st>>>(
-        (const T*)table, stride, rows, dim, index, index_bytes, count * dim, scale, (T*)out);
+  const bool rows16 = (reinterpret_cast<uintptr_t>(table) & 15) == 0 && dim % N == 0 &&
+                      stride % N == 0;
+  const bool narrow = total + kLookThreads * kLookVecs * N < (int64_t(1) << 32);
+#define GO(I, A)                                                                          \
+  lookup_kernel<T, I, A><<<(unsigned)grid, kLookThreads, 0, st>>>(                        \
+      (const T*)table, stride, rows, (I)dim, index, index_bytes, (I)total, scale, (T*)out)
+  if (rows16) {
+    if (narrow) GO(uint32_t, true); else GO(int64_t, true);
+  } else {
+    if (narrow) GO(uint32_t, false); else GO(int64_t, false);
+  }
+#undef GO
   SINKSLOT_CHECK_LAUNCH();
   return kOk;
 }
@@ -180,6 +226,14 @@ __global__ void __launch_bounds__(256) lookup_key_kernel(const void* __restrict_
   if (t < count) keys[t] = key_of(index, index_bytes, t, rows, padding);
 }
 
+__global__ void __launch_bounds__(256) lookup_zip_kernel(const uint32_t* __restrict__ keys,
+                                                         const uint32_t* __restrict__ perm,
+                                                         int64_t count,
+                                                         uint2* __restrict__ items) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t < count) items[t] = make_uint2(keys[t], perm[t]);
+}
+
 // One cluster (the grid's first) sorts; the other CTAs write the table's zeros.
 // Least significant digit first, 9 bits a pass: the 18 bits of a table of 2^17
 // rows take two.  Each warp ranks a run of its CTA's tokens by digit (match, in
@@ -206,8 +260,7 @@ static size_t sort_smem(int per) { return sizeof(SortShared) + (size_t)per * 16;
 
 __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     const void* __restrict__ index, int index_bytes, int count, int64_t rows, int64_t padding,
-    int per, int bits, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ perm_out,
-    uint32_t* __restrict__ chains, uint4* __restrict__ zeros, int64_t zero_vecs,
+    int per, int bits, uint2* __restrict__ items, uint32_t* __restrict__ chains, uint4* __restrict__ zeros, int64_t zero_vecs,
     int64_t zero_tail) {
   cg::cluster_group cl = cg::this_cluster();
   const int split = (int)cl.num_blocks(), rank = (int)cl.block_rank();
@@ -221,7 +274,7 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
   }
   extern __shared__ __align__(16) unsigned char raw[];
   SortShared& sh = *reinterpret_cast<SortShared*>(raw);
-  uint32_t* buf = reinterpret_cast<uint32_t*>(raw + sizeof(SortShared));  // keys, values, twice
+  uint2* buf = reinterpret_cast<uint2*>(raw + sizeof(SortShared));  // (row, token) twice
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int mine = max(0, min(per, count - rank * per));
   const int run = per / kSortCtaWarps;  // a warp's tokens (per is a multiple of kSortCta)
@@ -232,24 +285,19 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     for (int i = threadIdx.x; i < kSortCtaWarps * kDigits / 2; i += kSortCta)
       reinterpret_cast<uint32_t*>(sh.warp_count)[i] = 0;
     __syncthreads();
-    uint32_t key[kSortRounds], val[kSortRounds];
+    uint2 item[kSortRounds];
     uint16_t loc[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
       if (r * 32 >= run) break;
       const int i = warp * run + r * 32 + lane;
       const bool on = i < mine;
-      key[r] = val[r] = 0;
-      if (on) {
-        if (shift == 0) {
-          val[r] = (uint32_t)(rank * per + i);
-          key[r] = key_of(index, index_bytes, rank * per + i, rows, padding);
-        } else {
-          key[r] = buf[cur * 2 * per + i];
-          val[r] = buf[cur * 2 * per + per + i];
-        }
-      }
-      const uint32_t dg = on ? (key[r] >> shift) & (kDigits - 1) : kDigits;
+      item[r] = make_uint2(0, 0);
+      if (on)
+        item[r] = shift == 0 ? make_uint2(key_of(index, index_bytes, rank * per + i, rows, padding),
+                                          (uint32_t)(rank * per + i))
+                             : buf[cur * per + i];
+      const uint32_t dg = on ? (item[r].x >> shift) & (kDigits - 1) : kDigits;
       const uint32_t peers = __match_any_sync(0xffffffffu, dg);
       const uint32_t before = __popc(peers & ((1u << lane) - 1u));
       uint32_t base = 0;
@@ -298,16 +346,13 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     for (int r = 0; r < kSortRounds; ++r) {
       if (r * 32 >= run) break;
       if (warp * run + r * 32 + lane < mine) {
-        const uint32_t dg = (key[r] >> shift) & (kDigits - 1);
+        const uint32_t dg = (item[r].x >> shift) & (kDigits - 1);
         const uint32_t pos = sh.base[dg] + sh.warp_count[warp][dg] + loc[r];
         if (last) {
-          keys_out[pos] = key[r];
-          perm_out[pos] = val[r];
+          items[pos] = item[r];
         } else {
           const uint32_t to = pos / (uint32_t)per, at = pos - to * (uint32_t)per;
-          uint32_t* dst = cl.map_shared_rank(buf, to) + (cur ^ 1) * 2 * per;
-          dst[at] = key[r];
-          dst[per + at] = val[r];
+          cl.map_shared_rank(buf, to)[(cur ^ 1) * per + at] = item[r];
         }
       }
     }
@@ -342,8 +387,7 @@ __global__ void __launch_bounds__(kLookThreads) lookup_zero_kernel(uint4* __rest
 constexpr int kAhead = 8;  // loads in flight per thread; windows are multiples of it
 
 struct SumArgs {
-  const uint32_t* keys;
-  const uint32_t* perm;
+  const uint2* items;  // (row, token), sorted
   int64_t count, rows, stride, dim, ncv;
   int window;
   float scale;
@@ -437,14 +481,14 @@ __global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
     const int64_t s1 =
         min(a.count, (((int64_t)blockIdx.x + 1) * kLookThreads - 1) / a.ncv * a.window + a.window);
     for (int64_t i = s0 + threadIdx.x; i < s1; i += kLookThreads)
-      staged[i - s0] = make_uint2(a.keys[i], a.perm[i]);
+      staged[i - s0] = a.items[i];
     __syncthreads();
   }
   auto entry = [&](int64_t i) {
     if constexpr (kStage)
       return staged[i - s0];
     else
-      return make_uint2(a.keys[i], a.perm[i]);
+      return a.items[i];
   };
   chain_release();
   if (i0 >= a.count) return;
@@ -452,7 +496,7 @@ __global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
   uint32_t cur = entry(i0).x;
   if (cur >= a.rows) return;
   const T* gend = g + (a.count - 1) * a.stride + a.dim;
-  bool head = i0 > 0 && a.keys[i0 - 1] == cur;
+  bool head = i0 > 0 && a.items[i0 - 1].x == cur;
   float acc[VN];
 #pragma unroll
   for (int k = 0; k < VN; ++k) acc[k] = 0.0f;
@@ -471,16 +515,7 @@ __global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
         } else if constexpr (kAligned) {
           u[k] = __ldg(reinterpret_cast<const uint4*>(p) + j);
         } else {
-          const int64_t c = first_column<T, VN>(out + (int64_t)key[k] * a.dim, j);
-          if (c >= 0 && c + VN <= a.dim) {
-            u[k] = load16(p + c, g, gend);
-          } else {
-            T t[VN];
-#pragma unroll
-            for (int m = 0; m < VN; ++m)
-              t[m] = c + m >= 0 && c + m < a.dim ? p[c + m] : from_f32<T>(0.0f);
-            memcpy(&u[k], t, 16);
-          }
+          u[k] = load16(p + first_column<T, VN>(out + (int64_t)key[k] * a.dim, j), g, gend);
         }
       }
     }
@@ -505,7 +540,7 @@ __global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
       }
     }
   }
-  if (!head && i0 + n < a.count && a.keys[i0 + n] == cur) {
+  if (!head && i0 + n < a.count && a.items[i0 + n].x == cur) {
     store_part<VN>(part_at<VN>(a, 2 * w + 1, j), acc);
     // (the order of the list decides nothing but who joins which row)
     if (j == 0) a.chains[1 + atomicAdd(a.chains, 1u)] = (uint32_t)w;
@@ -528,13 +563,13 @@ __global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a,
   const int64_t windows = (a.count + a.window - 1) / a.window;
   for (uint32_t item = blockIdx.x; item < chains; item += gridDim.x) {
     const int64_t w = a.chains[1 + item];
-    const uint32_t cur = a.keys[(w + 1) * a.window - 1];
+    const uint32_t cur = a.items[(w + 1) * a.window - 1].x;
     // the first window after w that does not begin with this row: 32 probes a step
     int64_t lo = w + 1, hi = windows;  // lo begins with it; the answer is in (lo, hi]
     while (hi - lo > 1) {
       const int64_t step = (hi - lo + 31) / 32;
       const int64_t at = lo + step * (lane + 1);
-      const bool same = at < hi && a.keys[at * a.window] == cur;
+      const bool same = at < hi && a.items[at * a.window].x == cur;
       const int found = __popc(__ballot_sync(0xffffffffu, same));  // a prefix of the lanes
       const int64_t next = lo + step * (found + 1);
       lo += step * found;
@@ -583,6 +618,7 @@ static int window_of(int64_t count, int64_t dim) {
 }
 
 struct LookWs {
+  uint2* items;
   uint32_t *k1, *v1, *k2, *v2, *chains;
   int64_t *hist, *stmp;
   float* part;
@@ -592,10 +628,11 @@ static void carve_look(Carver& cv, LookWs& w, int64_t count, int64_t dim) {
   const int64_t e = count > 0 ? count : 1;
   const int64_t windows = ceil_div64(e, window_of(e, dim));
   w.chains = cv.take<uint32_t>(windows + 1);
-  w.k1 = cv.take<uint32_t>(e); w.v1 = cv.take<uint32_t>(e);
-  w.k2 = w.v2 = nullptr;
+  w.items = cv.take<uint2>(e);
+  w.k1 = w.v1 = w.k2 = w.v2 = nullptr;
   w.hist = w.stmp = nullptr;
   if (e > kSortMost) {
+    w.k1 = cv.take<uint32_t>(e); w.v1 = cv.take<uint32_t>(e);
     w.k2 = cv.take<uint32_t>(e); w.v2 = cv.take<uint32_t>(e);
     const int64_t nh = radix_hist_elems(1, e);
     w.hist = cv.take<int64_t>(nh);
@@ -647,7 +684,7 @@ static int launch_sums_of(SumArgs a, const void* g, void* out, cudaStream_t st) 
 // Sorts the tokens and writes the table's zeros.
 static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_t rows,
                        int64_t padding, void* out, int64_t out_bytes, LookWs& w,
-                       const uint32_t** keys, const uint32_t** perm, cudaStream_t st) {
+                       cudaStream_t st) {
   const int bits = bits_for((uint64_t)rows + 1);
   if (count > kSortMost) {
     SINKSLOT_CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)out_bytes, st));
@@ -658,8 +695,9 @@ static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_
     bool alt = false;
     SINKSLOT_TRY(radix_sort_pairs<uint32_t>(w.k1, w.v1, w.k2, w.v2, true, 1, count, bits, w.hist,
                                             w.stmp, &alt, st));
-    *keys = alt ? w.k2 : w.k1;
-    *perm = alt ? w.v2 : w.v1;
+    lookup_zip_kernel<<<(unsigned)ceil_div64(count, 256), 256, 0, st>>>(
+        alt ? w.k2 : w.k1, alt ? w.v2 : w.v1, count, w.items);
+    SINKSLOT_CHECK_LAUNCH();
     return kOk;
   }
   int split = 1;
@@ -695,16 +733,14 @@ static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   SINKSLOT_CUDA_TRY(cudaLaunchKernelEx(
-      &cfg, lookup_sort_kernel, index, index_bytes, (int)count, rows, padding, per, bits, w.k1,
-      w.v1, w.chains, (uint4*)out, vecs, tail));
+      &cfg, lookup_sort_kernel, index, index_bytes, (int)count, rows, padding, per, bits,
+      w.items, w.chains, (uint4*)out, vecs, tail));
   if (apart) {
     const int64_t grid = ceil_div64(vecs, kLookThreads * kFillVecs);
     SINKSLOT_REQUIRE(grid <= 0x7fffffff, "lookup_grad: sizes too large");
     SINKSLOT_CUDA_TRY(launch_chained(lookup_zero_kernel, dim3((unsigned)grid), dim3(kLookThreads),
                                      0, st, (uint4*)out, vecs, tail));
   }
-  *keys = w.k1;
-  *perm = w.v1;
   return kOk;
 }
 
@@ -735,7 +771,8 @@ int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* ind
   }
   SumArgs a = {};
   SINKSLOT_TRY(sort_tokens(index, index_bytes, count, rows, padding, grad_table, out_bytes, w,
-                           &a.keys, &a.perm, st));
+                           st));
+  a.items = w.items;
   a.count = count;
   a.rows = rows;
   a.stride = stride;

@@ -251,7 +251,7 @@ def _check_lookup(sk, table, index, scale, padding=None):
                                              (5, 8, 32), (1000, 64, 33), (50, 771, 4097),
                                              (9000, 1032, 700), (2, 257, 20000), (70000, 24, 5000),
                                              (300, 4100, 64), (150000, 5, 90112),
-                                             (600, 9, 90113), (1 << 20, 2, 200001), (40, 40, 65000)])
+                                             (600, 9, 90113), (30, 7, 1001), (9, 11, 515), (1 << 20, 2, 200001), (40, 40, 65000)])
 def test_lookup_sizes(sk, rows, dim, tokens, dtype):
     gen = _gen(rows + dim + tokens)
     table = torch.randn(rows, dim, generator=gen, device="cuda").to(dtype)
