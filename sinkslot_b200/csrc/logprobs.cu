@@ -53,22 +53,36 @@ __device__ __forceinline__ void rebase(Online& o, float m2, Scale2 c) {
   o.m = m2;
 }
 
-template <bool kEnt, int N>
-__device__ __forceinline__ void absorb(Online& o, const float (&f)[N], Scale2 c) {
-  float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+// Adds the elements of U vectors, none of them above o.m.  Two elements for each
+// instruction but the exponential: five instructions an element otherwise kept the
+// pass from the memory's rate.
+template <typename T, bool kEnt, int U>
+__device__ __forceinline__ void absorb(Online& o, const uint4 (&u)[U], Scale2 c) {
+  constexpr int N = Vec16<T>::N;
+  const f32x2 nm = pair(-o.m, -o.m), hi = pair(c.hi, c.hi), lo = pair(c.lo, c.lo);
+  f32x2 s = pair(0.0f, 0.0f), w = s;
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float d0 = f[i] - o.m, d1 = f[i + 1] - o.m;
-    const float e0 = exp_scaled(d0, c), e1 = exp_scaled(d1, c);
-    s0 += e0;
-    s1 += e1;
-    if (kEnt) {  // exp(-inf) * -inf counts as 0
-      w0 = fmaf(e0, fmaxf(d0, -1e30f), w0);
-      w1 = fmaf(e1, fmaxf(d1, -1e30f), w1);
+  for (int k = 0; k < U; ++k) {
+    float f[N];
+    unpack(u[k], f, (const T*)nullptr);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const f32x2 d = add2(pair(f[i], f[i + 1]), nm);
+      const float2 x = parts(fma2(d, hi, mul2(d, lo)));
+      const f32x2 e = pair(exp2_fast(x.x), exp2_fast(x.y));
+      s = add2(s, e);
+      if (kEnt) {  // exp(-inf) * -inf counts as 0
+        const float2 t = parts(d);
+        w = fma2(e, pair(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), w);
+      }
     }
   }
-  o.s += s0 + s1;
-  if (kEnt) o.w += w0 + w1;
+  const float2 a = parts(s);
+  o.s += a.x + a.y;
+  if (kEnt) {
+    const float2 b = parts(w);
+    o.w += b.x + b.y;
+  }
 }
 
 template <bool kEnt>
@@ -98,49 +112,42 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64
                     : (int64_t) static_cast<const int32_t*>(tokens)[r];
 }
 
-// Reads elements [rank's share] of one row into `o`.  `lane` of `lanes` threads.
+// Reads this CTA's share of a row (`rank` of `split`) into `o`, as thread `lane` of
+// `lanes`: rounds of kRowUnroll vectors, then vector by vector, then the elements
+// before the first boundary and behind the last.
 template <typename T, bool kEnt>
 __device__ __forceinline__ void read_row(Online& o, const T* __restrict__ p, int64_t vocab,
-                                         int lane, int lanes, int rank, int split,
-                                         Scale2 c) {
+                                         int lane, int lanes, int rank, int split, Scale2 c) {
   constexpr int N = Vec16<T>::N;
   const RowSpan sp = row_span(p, vocab);
-  const uint4* body = reinterpret_cast<const uint4*>(p + sp.head);
-  const int64_t share = (sp.body + split - 1) / split;
-  const int64_t v1 = min(sp.body, share * (rank + 1));
-  for (int64_t i = share * rank + lane; i < v1; i += (int64_t)lanes * kRowUnroll) {
+  const int body = (int)sp.body, share = (body + split - 1) / split;
+  const int v0 = min(body, share * rank), v1 = min(body, v0 + share);
+  const uint4* at = reinterpret_cast<const uint4*>(p + sp.head) + v0 + lane;
+  int left = v1 - v0 - lane;  // vectors from `at` on, of which every lanes-th is this thread's
+  for (; left > (kRowUnroll - 1) * lanes; left -= kRowUnroll * lanes, at += kRowUnroll * lanes) {
     uint4 u[kRowUnroll];
 #pragma unroll
-    for (int k = 0; k < kRowUnroll; ++k) {
-      const int64_t at = i + (int64_t)k * lanes;
-      if (at < v1) u[k] = __ldg(body + at);
-    }
-    float f[kRowUnroll][N];
-    float mx = -FLT_MAX;
+    for (int k = 0; k < kRowUnroll; ++k) u[k] = __ldg(at + k * lanes);
+    float mx = max_of(u[0], (const T*)nullptr);
 #pragma unroll
-    for (int k = 0; k < kRowUnroll; ++k) {
-      if (i + (int64_t)k * lanes < v1) {
-        unpack(u[k], f[k], (const T*)nullptr);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[k][j] = -INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) mx = fmaxf(mx, f[k][j]);
-    }
+    for (int k = 1; k < kRowUnroll; ++k) mx = fmaxf(mx, max_of(u[k], (const T*)nullptr));
     rebase<kEnt>(o, fmaxf(o.m, mx), c);
-#pragma unroll
-    for (int k = 0; k < kRowUnroll; ++k) absorb<kEnt>(o, f[k], c);
+    absorb<T, kEnt>(o, u, c);
+  }
+  for (; left > 0; left -= lanes, at += lanes) {
+    const uint4 u[1] = {__ldg(at)};
+    rebase<kEnt>(o, fmaxf(o.m, max_of(u[0], (const T*)nullptr)), c);
+    absorb<T, kEnt>(o, u, c);
   }
   if (rank == 0) {
     const int64_t tail0 = sp.head + sp.body * N;
-    const int64_t edge = sp.head + (vocab - tail0);
-    for (int64_t e = lane; e < edge; e += lanes) {
-      float f[2];
-      f[0] = to_f32(p[e < sp.head ? e : tail0 + e - sp.head]);
-      f[1] = -INFINITY;
-      rebase<kEnt>(o, fmaxf(o.m, f[0]), c);
-      absorb<kEnt>(o, f, c);
+    const int edge = (int)(sp.head + (vocab - tail0));
+    for (int e = lane; e < edge; e += lanes) {
+      const float f = to_f32(p[e < sp.head ? e : tail0 + e - sp.head]);
+      rebase<kEnt>(o, fmaxf(o.m, f), c);
+      const float d = f - o.m, x = exp_scaled(d, c);
+      o.s += x;
+      if (kEnt) o.w = fmaf(x, fmaxf(d, -1e30f), o.w);
     }
   }
 }
@@ -250,6 +257,7 @@ static Scale2 scale2(double inv_temp) {
 static int check_rows(const LogitRows& r) {
   SINKSLOT_REQUIRE(dtype_ok(r.dtype), "token_logprobs: dtype must be 0, 1 or 2");
   SINKSLOT_REQUIRE(r.rows >= 0 && r.vocab >= 1 && r.stride >= 0, "token_logprobs: bad sizes");
+  SINKSLOT_REQUIRE(r.vocab <= int64_t(1) << 30, "token_logprobs: more than 2^30 tokens to choose");
   SINKSLOT_REQUIRE(r.token_bytes == 4 || r.token_bytes == 8,
                    "token_logprobs: tokens must be int32 or int64");
   SINKSLOT_REQUIRE(r.inv_temp >= 0.99e-30 && r.inv_temp <= 1.01e30,
@@ -318,8 +326,7 @@ struct RowCoef {
   float m, c;       // exponent: (z - m) * c
   float cp, ce, k;  // d = e * (cp + ce * ((z - m) * inv_temp + k))
   float inv_temp;
-  float hit;        // added at the token
-  int64_t tok;
+  float hit;  // added at the token
 };
 
 template <bool kEnt>
@@ -331,91 +338,132 @@ __device__ __forceinline__ float grad_at(float z, const RowCoef& q) {
 }
 
 template <typename T, bool kEnt>
-__global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogitRows r, LogitGrad g,
-                                                                   int64_t share) {
+__device__ __forceinline__ uint4 grad_vec(const uint4& u, const RowCoef& q) {
   constexpr int N = Vec16<T>::N;
+  float f[N];
+  unpack(u, f, (const T*)nullptr);
+  const f32x2 nm = pair(-q.m, -q.m), c = pair(q.c, q.c), cp = pair(q.cp, q.cp);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const f32x2 d = add2(pair(f[i], f[i + 1]), nm);
+    const float2 x = parts(mul2(d, c));
+    const f32x2 e = pair(exp2_fast(x.x), exp2_fast(x.y));
+    float2 r;
+    if (!kEnt) {
+      r = parts(mul2(e, cp));
+    } else {
+      const float2 t = parts(d);
+      const f32x2 l = fma2(pair(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)),
+                           pair(q.inv_temp, q.inv_temp), pair(q.k, q.k));
+      r = parts(mul2(e, fma2(pair(q.ce, q.ce), l, cp)));
+    }
+    f[i] = r.x;
+    f[i + 1] = r.y;
+  }
+  return pack(f, (const T*)nullptr);
+}
+
+// Writes the gradient of vectors [v0, v1) of a row (cut by the output's 16-byte
+// boundaries) and, where `edges`, of the elements around its vectors.
+// same: the logits' row lies on the output's phase.
+template <typename T, bool kEnt>
+__device__ __forceinline__ void write_grad(const T* __restrict__ p, T* __restrict__ out,
+                                           int64_t vocab, int v0, int v1, bool edges, bool same,
+                                           int lane, int lanes, int64_t tok, const RowCoef& q) {
+  constexpr int N = Vec16<T>::N;
+  const RowSpan sp = row_span(out, vocab);
+  uint4* ob = reinterpret_cast<uint4*>(out + sp.head) + v0 + lane;
+  const T* first = p + sp.head + ((int64_t)v0 + lane) * N;
+  int left = v1 - v0 - lane;
+  if (same) {
+    const uint4* ib = reinterpret_cast<const uint4*>(first);
+    for (; left > (kRowUnroll - 1) * lanes;
+         left -= kRowUnroll * lanes, ib += kRowUnroll * lanes, ob += kRowUnroll * lanes) {
+      uint4 u[kRowUnroll];
+#pragma unroll
+      for (int k = 0; k < kRowUnroll; ++k) u[k] = __ldg(ib + k * lanes);
+#pragma unroll
+      for (int k = 0; k < kRowUnroll; ++k) __stcs(ob + k * lanes, grad_vec<T, kEnt>(u[k], q));
+    }
+    for (; left > 0; left -= lanes, ib += lanes, ob += lanes)
+      __stcs(ob, grad_vec<T, kEnt>(__ldg(ib), q));
+  } else {
+    for (; left > 0; left -= lanes, first += (int64_t)lanes * N, ob += lanes) {
+      T t[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) t[j] = first[j];
+      uint4 u;
+      memcpy(&u, t, 16);
+      *ob = grad_vec<T, kEnt>(u, q);
+    }
+  }
+  const int64_t tail0 = sp.head + sp.body * N;
+  if (edges) {
+    const int edge = (int)(sp.head + (vocab - tail0));
+    for (int e = lane; e < edge; e += lanes) {
+      const int64_t at = e < sp.head ? e : tail0 + e - sp.head;
+      out[at] = from_f32<T>(grad_at<kEnt>(to_f32(p[at]), q) + (at == tok ? q.hit : 0.0f));
+    }
+  }
+  // the token's own element, by the thread that wrote its vector
+  if (tok >= sp.head && tok < tail0) {
+    const int64_t tv = (tok - sp.head) / N;
+    if (tv >= v0 && tv < v1 && (tv - v0) % lanes == lane)
+      out[tok] = from_f32<T>(grad_at<kEnt>(to_f32(p[tok]), q) + q.hit);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_zeros(T* __restrict__ out, int64_t vocab, int v0, int v1,
+                                            bool edges, int lane, int lanes) {
+  const RowSpan sp = row_span(out, vocab);
+  uint4* ob = reinterpret_cast<uint4*>(out + sp.head);
+  for (int i = v0 + lane; i < v1; i += lanes) __stcs(ob + i, make_uint4(0, 0, 0, 0));
+  if (!edges) return;
+  const int64_t tail0 = sp.head + sp.body * Vec16<T>::N;
+  const int edge = (int)(sp.head + (vocab - tail0));
+  for (int e = lane; e < edge; e += lanes)
+    out[e < sp.head ? e : tail0 + e - sp.head] = from_f32<T>(0.0f);
+}
+
+// 1 / s, 0 for a row of nothing but -inf (no gradient), NaN for NaN.
+__device__ __forceinline__ float inverse_sum(float s) {
+  return s > 0.0f ? 1.0f / s : (s == 0.0f ? 0.0f : s);
+}
+
+template <typename T, bool kEnt>
+__global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogitRows r, LogitGrad g,
+                                                                   int share) {
   const int64_t row = blockIdx.x;
   const int64_t tok = token_at(r.tokens, r.token_bytes, row);
-  const bool skip = tok == r.ignore || (r.mask && !r.mask[row]);
   const T* p = static_cast<const T*>(r.z) + row * r.stride;
   T* out = static_cast<T*>(g.dz) + row * g.dz_stride;
-  // vectors are cut by the output's boundaries; the input's may lie elsewhere
-  const RowSpan sp = row_span(out, r.vocab);
-  const bool same = !((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(out)) & 15);
-  const int64_t v0 = share * blockIdx.y, v1 = min(sp.body, v0 + share);
-  uint4* ob = reinterpret_cast<uint4*>(out + sp.head);
-  const T* ib = p + sp.head;
-  const int64_t tail0 = sp.head + sp.body * N;
-  const int64_t edge = blockIdx.y == 0 ? sp.head + (r.vocab - tail0) : 0;
-  if (skip) {
-    for (int64_t i = v0 + threadIdx.x; i < v1; i += kRowThreads) ob[i] = make_uint4(0, 0, 0, 0);
-    for (int64_t e = threadIdx.x; e < edge; e += kRowThreads)
-      out[e < sp.head ? e : tail0 + e - sp.head] = from_f32<T>(0.0f);
+  const int body = (int)row_span(out, r.vocab).body;
+  const int v0 = min(body, share * (int)blockIdx.y), v1 = min(body, v0 + share);
+  const bool edges = blockIdx.y == 0;
+  if (tok == r.ignore || (r.mask && !r.mask[row])) {
+    write_zeros(out, r.vocab, v0, v1, edges, threadIdx.x, kRowThreads);
     return;
   }
   RowCoef q;
-  {
-    const float2 ms = g.stats[row];
-    const float inv_temp = (float)r.inv_temp;
-    float f = inv_temp * g.scale;
-    if (g.scale_dev) f *= g.scale_dev[0];
-    const float gp = g.g ? g.g[row * g.g_stride] * f : 0.0f;
-    const float rs = ms.y > 0.0f ? 1.0f / ms.y : (ms.y == 0.0f ? 0.0f : ms.y);
-    q.m = ms.x;
-    q.c = (float)(r.inv_temp * 1.4426950408889634);
-    q.inv_temp = inv_temp;
-    q.cp = -gp * rs;
-    q.ce = q.k = 0.0f;
-    if (kEnt) {
-      const float ge = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] * f : 0.0f;
-      q.ce = -ge * rs;
-      q.k = ms.y > 0.0f ? g.entropy[row] - logf(ms.y) : 0.0f;
-    }
-    q.hit = gp;
-    q.tok = tok;
+  const float2 ms = g.stats[row];
+  q.inv_temp = (float)r.inv_temp;
+  float f = q.inv_temp * g.scale;
+  if (g.scale_dev) f *= g.scale_dev[0];
+  const float gp = g.g ? g.g[row * g.g_stride] * f : 0.0f;
+  const float rs = inverse_sum(ms.y);
+  q.m = ms.x;
+  q.c = (float)(r.inv_temp * 1.4426950408889634);
+  q.cp = -gp * rs;
+  q.ce = q.k = 0.0f;
+  if (kEnt) {
+    const float ge = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] * f : 0.0f;
+    q.ce = -ge * rs;
+    q.k = ms.y > 0.0f ? g.entropy[row] - logf(ms.y) : 0.0f;
   }
-  const bool empty = g.stats[row].y == 0.0f;  // every logit is -inf: no gradient
-  if (empty) q.hit = 0.0f;
-  const int64_t tv = q.tok >= sp.head && q.tok < tail0 ? (q.tok - sp.head) / N : -1;
-  for (int64_t i = v0 + threadIdx.x; i < v1; i += (int64_t)kRowThreads * kRowUnroll) {
-    uint4 u[kRowUnroll];
-#pragma unroll
-    for (int k = 0; k < kRowUnroll; ++k) {
-      const int64_t at = i + (int64_t)k * kRowThreads;
-      if (at < v1) {
-        if (same) {
-          u[k] = __ldg(reinterpret_cast<const uint4*>(ib) + at);
-        } else {
-          T t[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) t[j] = ib[at * N + j];
-          memcpy(&u[k], t, 16);
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kRowUnroll; ++k) {
-      const int64_t at = i + (int64_t)k * kRowThreads;
-      if (at < v1) {
-        float f[N];
-        unpack(u[k], f, (const T*)nullptr);
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = grad_at<kEnt>(f[j], q);
-        if (at == tv) {
-          const int jt = (int)(q.tok - sp.head - at * N);
-#pragma unroll
-          for (int j = 0; j < N; ++j) f[j] += j == jt ? q.hit : 0.0f;
-        }
-        ob[at] = pack(f, (const T*)nullptr);
-      }
-    }
-  }
-  for (int64_t e = threadIdx.x; e < edge; e += kRowThreads) {
-    const int64_t at = e < sp.head ? e : tail0 + e - sp.head;
-    float f = grad_at<kEnt>(to_f32(p[at]), q);
-    if (at == q.tok) f += q.hit;
-    out[at] = from_f32<T>(f);
-  }
+  q.hit = ms.y == 0.0f ? 0.0f : gp;
+  const bool same = !((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(out)) & 15);
+  write_grad<T, kEnt>(p, out, r.vocab, v0, v1, edges, same, threadIdx.x, kRowThreads, tok, q);
 }
 
 template <typename T>
@@ -428,7 +476,7 @@ static int launch_grad(const LogitRows& r, const LogitGrad& g, cudaStream_t st) 
   if (pieces > ceil_div64(body, least)) pieces = ceil_div64(body, least);
   if (pieces < 1) pieces = 1;
   if (pieces > 65535) pieces = 65535;
-  const int64_t share = ceil_div64(body, pieces);
+  const int share = (int)ceil_div64(body, pieces);
   const dim3 grid((unsigned)r.rows, (unsigned)pieces);
   if (g.g_entropy)
     logprob_grad_kernel<T, true><<<grid, kRowThreads, 0, st>>>(r, g, share);

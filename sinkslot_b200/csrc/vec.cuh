@@ -71,6 +71,56 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two floats in one 64-bit register and the arithmetic that sm_100 has on them.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// The largest element of a vector (NaNs count as nothing: the sum shows them).
+__device__ __forceinline__ float max_of(const uint4& u, const float*) {
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+__device__ __forceinline__ float max_of(const uint4& u, const __half*) {
+  const __half2 a = __hmax2(*reinterpret_cast<const __half2*>(&u.x),
+                            *reinterpret_cast<const __half2*>(&u.y));
+  const __half2 b = __hmax2(*reinterpret_cast<const __half2*>(&u.z),
+                            *reinterpret_cast<const __half2*>(&u.w));
+  const float2 t = __half22float2(__hmax2(a, b));
+  return fmaxf(t.x, t.y);
+}
+__device__ __forceinline__ float max_of(const uint4& u, const __nv_bfloat16*) {
+  const __nv_bfloat162 a = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&u.x),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  const __nv_bfloat162 b = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&u.z),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&u.w));
+  const float2 t = __bfloat1622float2(__hmax2(a, b));
+  return fmaxf(t.x, t.y);
+}
+
 // A row of n elements from p: `head` elements up to the first 16-byte boundary,
 // `body` whole vectors, then the rest.
 struct RowSpan {
