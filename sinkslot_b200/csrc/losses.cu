@@ -379,28 +379,85 @@ int scale_tokens(const float* coef, int64_t tokens, const float* norm, const flo
 }
 
 // --------------------------------------------------------------------------
-// Policy loss from the logits: log-probabilities, token terms, logits' gradient.
+// Policy loss from the logits.  Where they are larger than L2, one pass over the
+// rows gives log-probabilities and gradient (policy_rows.cu: the logits are read
+// from memory once); it needs the counts of the whole batch first.  Others go
+// through the log-probabilities' own kernels.
 // --------------------------------------------------------------------------
+
+// Counts, and the sequence of each token (-1: none).
+__global__ void __launch_bounds__(kLossThreads) policy_count_kernel(Packed p, int split,
+                                                                    int64_t* __restrict__ counts,
+                                                                    int* __restrict__ owner) {
+  __shared__ ClusterSum sh;
+  const int64_t seq = blockIdx.x / (unsigned)split;
+  const int rank = (int)(blockIdx.x % (unsigned)split);
+  const int64_t at = (int64_t)rank * kLossThreads + threadIdx.x;
+  const int64_t step = (int64_t)split * kLossThreads;
+  int64_t lo, hi, n = 0;
+  bounds(p, seq, lo, hi);
+  for (int64_t i = lo + at; i < hi; i += step) {
+    n += !p.mask || p.mask[i];
+    owner[i] = (int)seq;
+  }
+  if (p.offsets && seq == 0)
+    for (int64_t i = at, e = offset_at(p, 0); i < e; i += step) owner[i] = -1;
+  if (p.offsets && seq == p.count - 1)
+    for (int64_t i = offset_at(p, p.count) + at; i < p.tokens; i += step) owner[i] = -1;
+  const Sums f = cluster_sums({(double)n, 0.0, 0.0}, sh, 0, rank, split);
+  if (rank == 0 && threadIdx.x == 0) counts[seq] = (int64_t)f.a;
+  chain_release();
+}
+
+__global__ void __launch_bounds__(kLossThreads) policy_norm_kernel(
+    const int64_t* __restrict__ counts, int64_t count, int by_sequence, float* __restrict__ norm) {
+  __shared__ ClusterSum sh;
+  chain_enter();
+  Sums k = {0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < count; i += kLossThreads)
+    k.a += by_sequence ? (counts[i] > 0 ? 1.0 : 0.0) : (double)counts[i];
+  k = cta_sums(k, sh, 0);
+  if (threadIdx.x == 0) norm[0] = k.a > 0.0 ? (float)(1.0 / k.a) : 0.0f;
+}
+
 size_t policy_logits_workspace_bytes(int64_t rows, int64_t count) {
   const size_t r = (size_t)(rows > 0 ? rows : 1);
-  return loss_workspace_bytes(count) + align_up(r * sizeof(float2)) + align_up(r * sizeof(float));
+  return loss_workspace_bytes(count) + align_up(r * sizeof(float2)) + align_up(r * sizeof(float)) +
+         align_up((size_t)count * sizeof(int64_t)) + align_up(sizeof(float));
 }
 
 int policy_loss_logits(const LogitRows& r, const Packed& p, const PolicyTerms& t, float grad_scale,
                        float* values, float* logp, void* dz, int64_t dz_stride, void* ws,
                        size_t ws_bytes, cudaStream_t st) {
   SINKSLOT_REQUIRE(p.tokens == r.rows, "policy_loss_from_logits: bad sizes");
+  SINKSLOT_TRY(check_packed(p));
   Carver cv(ws, ws_bytes);
   float2* stats = cv.take<float2>((size_t)(r.rows > 0 ? r.rows : 1));
   float* coef = cv.take<float>((size_t)(r.rows > 0 ? r.rows : 1));
   char* part = cv.take<char>(loss_workspace_bytes(p.count));
+  int64_t* counts = cv.take<int64_t>((size_t)p.count);
+  float* norm = cv.take<float>(1);
   if (!cv.ok) {
     set_error("policy_loss_from_logits: workspace too small");
     return kWorkspaceTooSmall;
   }
-  SINKSLOT_TRY(token_logprobs(r, logp, nullptr, stats, st));
   PolicyTerms u = t;
   u.logp = logp;
+  if (dz && r.rows > 0 && policy_rows_fit(r, dz, dz_stride)) {
+    const int split = loss_split(p);
+    int* owner = reinterpret_cast<int*>(coef);
+    SINKSLOT_CUDA_TRY(launch_cluster(policy_count_kernel, p.count, split, kLossThreads, st, p,
+                                     split, counts, owner));
+    SINKSLOT_CUDA_TRY(launch_chained(policy_norm_kernel, dim3(1), dim3(kLossThreads), 0, st,
+                                     (const int64_t*)counts, p.count, t.sequence_average, norm));
+    PolicyRows w;
+    w.owner = owner;
+    w.counts = counts;
+    w.norm = norm;
+    SINKSLOT_TRY(policy_rows(r, u, w, grad_scale, logp, dz, dz_stride, st));
+    return policy_loss(p, u, values, nullptr, part, loss_workspace_bytes(p.count), st);
+  }
+  SINKSLOT_TRY(token_logprobs(r, logp, nullptr, stats, st));
   SINKSLOT_TRY(policy_loss(p, u, values, dz ? coef : nullptr, part, loss_workspace_bytes(p.count),
                            st));
   if (!dz || r.rows == 0) return kOk;

@@ -31,11 +31,11 @@ struct TokenTerm {
 
 // One token's loss, KL estimate and d loss / d logp.  The clip is decided on the
 // difference of the log-probabilities in fp64, which is exact.
-__device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
-                                                 float logp, int64_t at, int64_t seq) {
+__device__ __forceinline__ TokenTerm policy_term_of(const PolicyTerms& t, const PolicyEdges& e,
+                                                    float logp, float old_logp, float ref_logp,
+                                                    float adv) {
   TokenTerm o;
-  const double d = (double)logp - (double)t.old_logp[at];
-  const float adv = t.adv[t.adv_per_token ? at : seq];
+  const double d = (double)logp - (double)old_logp;
   const bool over = d > e.over, under = d < e.under;
   const float r = expf((float)d);
   const float rc = over ? e.rhi : (under ? e.rlo : r);
@@ -45,7 +45,7 @@ __device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const Pol
   o.coef = o.clipped ? 0.0f : -r * adv;
   o.kl = 0.0f;
   if (t.ref_logp) {
-    const float g = (float)((double)t.ref_logp[at] - (double)logp);
+    const float g = (float)((double)ref_logp - (double)logp);
     float slope;
     if (t.kl_kind == 1) {
       o.kl = -g;
@@ -63,6 +63,12 @@ __device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const Pol
     }
   }
   return o;
+}
+
+__device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
+                                                 float logp, int64_t at, int64_t seq) {
+  return policy_term_of(t, e, logp, t.old_logp[at], t.ref_logp ? t.ref_logp[at] : 0.0f,
+                        t.adv[t.adv_per_token ? at : seq]);
 }
 
 inline PolicyEdges policy_edges(const PolicyTerms& t) {

@@ -78,6 +78,17 @@ struct PolicyTerms {
   int kl_kind = 3;           // 1, 2, 3
   int sequence_average = 0;  // 0: mean over tokens, 1: mean of the sequences' means
 };
+// What a row's gradient needs of the whole batch: the sequence of each token (-1:
+// none), the sequences' counted tokens, and one over what the loss is averaged by.
+struct PolicyRows {
+  const int* owner = nullptr;
+  const int64_t* counts = nullptr;
+  const float* norm = nullptr;
+};
+// ---- policy_rows.cu: all rows' log-probabilities and gradient in one pass.
+bool policy_rows_fit(const LogitRows& r, const void* dz, int64_t dz_stride);
+int policy_rows(const LogitRows& r, const PolicyTerms& t, const PolicyRows& w, float grad_scale,
+                float* logp, void* dz, int64_t dz_stride, cudaStream_t st);
 struct PreferenceTerms {
   const float* logp = nullptr;
   const float* ref_logp = nullptr;  // nullable

@@ -456,7 +456,10 @@ def test_clip_is_decided_at_its_border(sk):
 @pytest.mark.parametrize("t,vocab,count,average,pad", [
     (1, 17, 0, "token", 0), (40, 333, 3, "sequence", 5), (64, 50021, 3, "sequence", 0),
     (9, 32768, 2, "token", 64), (700, 4099, 12, "token", 1), (300, 130000, 4, "sequence", 0),
-    (50, 262144, 1, "token", 0)])
+    (50, 262144, 1, "token", 0),
+    # logits larger than L2: rows that stay in shared memory, by 1, 2, 4 and 8 CTAs
+    (9100, 8233, 40, "sequence", 0), (2300, 32768, 5, "token", 64), (1400, 50021, 9, "sequence", 3),
+    (1200, 131072, 16, "token", 0)])
 def test_policy_loss_from_logits(sk, t, vocab, count, average, pad, dtype):
     gen = _gen(t + vocab)
     buf = (torch.randn(t, vocab + pad, generator=gen, device="cuda") * 2).to(dtype)
