@@ -17,7 +17,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
-#include "primitives.h"
+#include "primitives.h"  // bits_for
 #include "training.h"
 #include "vec.cuh"
 
@@ -218,22 +218,6 @@ __device__ __forceinline__ uint32_t key_of(const void* index, int bytes, int64_t
   return (uint32_t)(r < 0 || r >= rows || r == padding ? rows : r);
 }
 
-__global__ void __launch_bounds__(256) lookup_key_kernel(const void* __restrict__ index,
-                                                         int index_bytes, int64_t count,
-                                                         int64_t rows, int64_t padding,
-                                                         uint32_t* __restrict__ keys) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t < count) keys[t] = key_of(index, index_bytes, t, rows, padding);
-}
-
-__global__ void __launch_bounds__(256) lookup_zip_kernel(const uint32_t* __restrict__ keys,
-                                                         const uint32_t* __restrict__ perm,
-                                                         int64_t count,
-                                                         uint2* __restrict__ items) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t < count) items[t] = make_uint2(keys[t], perm[t]);
-}
-
 // One cluster (the grid's first) sorts; the other CTAs write the table's zeros.
 // Least significant digit first, 9 bits a pass: the 18 bits of a table of 2^17
 // rows take two.  Each warp ranks a run of its CTA's tokens by digit (match, in
@@ -358,6 +342,152 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     }
     // (the last pass as well: no CTA leaves while others read or write its memory)
     cl.sync();
+  }
+}
+
+// More tokens than a cluster holds: the same passes over tiles of kTile tokens, three
+// kernels each.  Digit counts of every tile; their sums over the tiles before (a warp
+// for each digit); tokens ranked within their tile, put in digit order in shared
+// memory and written out run by run.
+constexpr int kTileThreads = 512;
+constexpr int kTileWarps = kTileThreads / 32;
+constexpr int kTileRounds = 8;
+constexpr int kTile = kTileThreads * kTileRounds;
+
+struct TileSource {
+  const void* index;  // the first pass reads the indices, later ones the items
+  int index_bytes;
+  int64_t count, rows, padding;
+  const uint2* items;
+  int shift;
+};
+
+__device__ __forceinline__ uint2 tile_item(const TileSource& a, int64_t t) {
+  return a.items ? a.items[t]
+                 : make_uint2(key_of(a.index, a.index_bytes, t, a.rows, a.padding), (uint32_t)t);
+}
+
+__global__ void __launch_bounds__(kTileThreads) tile_count_kernel(TileSource a, int tiles,
+                                                                  uint32_t* __restrict__ counts) {
+  __shared__ uint32_t n[kDigits];
+  for (int i = threadIdx.x; i < kDigits; i += kTileThreads) n[i] = 0;
+  __syncthreads();
+  chain_enter();
+  chain_release();
+  const int64_t t0 = (int64_t)blockIdx.x * kTile + threadIdx.x;
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int64_t t = t0 + r * kTileThreads;
+    if (t < a.count) atomicAdd(&n[(tile_item(a, t).x >> a.shift) & (kDigits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kDigits; i += kTileThreads)
+    counts[(int64_t)i * tiles + blockIdx.x] = n[i];
+}
+
+__global__ void __launch_bounds__(256) tile_scan_kernel(uint32_t* __restrict__ counts, int tiles,
+                                                        uint32_t* __restrict__ totals) {
+  chain_enter();
+  chain_release();
+  const int digit = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  uint32_t* c = counts + (int64_t)digit * tiles;
+  uint32_t before = 0;
+  for (int k = 0; k < tiles; k += 32) {
+    const uint32_t v = k + lane < tiles ? c[k + lane] : 0;
+    uint32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (k + lane < tiles) c[k + lane] = before + incl - v;
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) totals[digit] = before;
+}
+
+// Sum of v over the threads before this one; kDigits threads, all of the CTA.
+__device__ __forceinline__ uint32_t digits_before(uint32_t v, uint32_t* warp_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int k = 0; k < warp; ++k) before += warp_sum[k];
+  return before + incl - v;
+}
+
+__global__ void __launch_bounds__(kTileThreads) tile_scatter_kernel(
+    TileSource a, int tiles, const uint32_t* __restrict__ counts,
+    const uint32_t* __restrict__ totals, uint2* __restrict__ out) {
+  static_assert(kTileThreads == kDigits, "a thread for each digit");
+  __shared__ uint2 sorted[kTile];  // before it, the warps' digit counts
+  uint16_t(*warp_count)[kDigits] = reinterpret_cast<uint16_t(*)[kDigits]>(sorted);
+  static_assert(sizeof(uint16_t) * kTileWarps * kDigits <= sizeof(uint2) * kTile, "fits");
+  __shared__ uint32_t begin[kDigits], global[kDigits], warp_sum[kTileWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < kTileWarps * kDigits / 2; i += kTileThreads)
+    reinterpret_cast<uint32_t*>(warp_count)[i] = 0;
+  __syncthreads();
+  chain_enter();
+  chain_release();
+  const int64_t t0 = (int64_t)blockIdx.x * kTile;
+  const int mine = (int)min((int64_t)kTile, a.count - t0);
+  uint2 item[kTileRounds];
+  uint16_t loc[kTileRounds];
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int i = warp * (kTile / kTileWarps) + r * 32 + lane;
+    item[r] = i < mine ? tile_item(a, t0 + i) : make_uint2(0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const bool on = warp * (kTile / kTileWarps) + r * 32 + lane < mine;
+    const uint32_t dg = on ? (item[r].x >> a.shift) & (kDigits - 1) : kDigits;
+    const uint32_t peers = __match_any_sync(0xffffffffu, dg);
+    const uint32_t before = __popc(peers & ((1u << lane) - 1u));
+    uint32_t base = 0;
+    if (on) base = warp_count[warp][dg];
+    __syncwarp();
+    if (on && before == 0) warp_count[warp][dg] = (uint16_t)(base + __popc(peers));
+    __syncwarp();
+    loc[r] = (uint16_t)(base + before);
+  }
+  __syncthreads();
+  {
+    const int d = threadIdx.x;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kTileWarps; ++w) {
+      const uint32_t c = warp_count[w][d];
+      warp_count[w][d] = (uint16_t)sum;
+      sum += c;
+    }
+    begin[d] = digits_before(sum, warp_sum);
+    global[d] = digits_before(totals[d], warp_sum) + counts[(int64_t)d * tiles + blockIdx.x];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r)
+    if (warp * (kTile / kTileWarps) + r * 32 + lane < mine) {
+      const uint32_t dg = (item[r].x >> a.shift) & (kDigits - 1);
+      loc[r] = (uint16_t)(begin[dg] + warp_count[warp][dg] + loc[r]);
+    }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r)
+    if (warp * (kTile / kTileWarps) + r * 32 + lane < mine) sorted[loc[r]] = item[r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine; i += kTileThreads) {
+    const uint2 v = sorted[i];
+    const uint32_t dg = (v.x >> a.shift) & (kDigits - 1);
+    out[global[dg] + (i - begin[dg])] = v;
   }
 }
 
@@ -549,62 +679,104 @@ __global__ void __launch_bounds__(kLookThreads) lookup_sum_kernel(SumArgs a,
   }
 }
 
-// Rows that cross windows: 32 chunks of columns for each CTA, its warps share the
-// row's windows in order and their sums are joined in order.
+// Rows that cross windows.  A warp takes a row and up to 32 chunks of its columns
+// (blockIdx.y): where there are fewer, its lanes share the row's windows as well.  Rows
+// over many windows are left to the CTA's warps together.  All sums are joined in an
+// order that the row's place alone decides.
+constexpr int kLongChain = 16;  // windows for each lane group of a warp
+
 template <typename T, int VN>
-__global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a,
+__global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a, int lanes,
                                                                    T* __restrict__ out) {
   constexpr int kWarps = kLookThreads / 32;
   __shared__ float sums[kWarps][32][VN + 1];
+  __shared__ uint32_t long_w[kWarps], long_n[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.y * 32 + lane;
-  chain_enter();
-  const uint32_t chains = a.chains[0];
-  const int64_t windows = (a.count + a.window - 1) / a.window;
-  for (uint32_t item = blockIdx.x; item < chains; item += gridDim.x) {
-    const int64_t w = a.chains[1 + item];
-    const uint32_t cur = a.items[(w + 1) * a.window - 1].x;
-    // the first window after w that does not begin with this row: 32 probes a step
-    int64_t lo = w + 1, hi = windows;  // lo begins with it; the answer is in (lo, hi]
-    while (hi - lo > 1) {
-      const int64_t step = (hi - lo + 31) / 32;
-      const int64_t at = lo + step * (lane + 1);
-      const bool same = at < hi && a.items[at * a.window].x == cur;
-      const int found = __popc(__ballot_sync(0xffffffffu, same));  // a prefix of the lanes
-      const int64_t next = lo + step * (found + 1);
-      lo += step * found;
-      if (next < hi) hi = next;
-    }
-    const int64_t n = hi - w;  // partial sums: w's tail, the heads of the windows behind
-    const int64_t k0 = n * warp / kWarps, k1 = n * (warp + 1) / kWarps;
-    float acc[VN];
-#pragma unroll
-    for (int m = 0; m < VN; ++m) acc[m] = 0.0f;
-    if (j < a.ncv) {
+  const int parts = 32 / lanes, mine = lane / lanes;  // lane groups, and this lane's
+  const int64_t j = (int64_t)blockIdx.y * 32 + lane % lanes;
+  const bool on = j < a.ncv;
+  // windows [k0, k1) of the row that begins in window w: w's tail, then heads
+  auto add = [&](float (&acc)[VN], int64_t w, int64_t k0, int64_t k1) {
 #pragma unroll 4
-      for (int64_t k = k0; k < k1; ++k) {
-        const float* p = part_at<VN>(a, 2 * (w + k) + (k == 0), j);
-        if constexpr (VN == 1) {
-          acc[0] += *p;
-        } else {
+    for (int64_t k = k0; k < k1; ++k) {
+      const float* p = part_at<VN>(a, 2 * (w + k) + (k == 0), j);
+      if constexpr (VN == 1) {
+        acc[0] += *p;
+      } else {
 #pragma unroll
-          for (int m = 0; m < VN; m += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + m);
-            acc[m] += v.x; acc[m + 1] += v.y; acc[m + 2] += v.z; acc[m + 3] += v.w;
-          }
+        for (int m = 0; m < VN; m += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p + m);
+          acc[m] += v.x; acc[m + 1] += v.y; acc[m + 2] += v.z; acc[m + 3] += v.w;
         }
       }
     }
-    __syncthreads();
+  };
+  auto over_groups = [&](float (&acc)[VN]) {
+    for (int d = lanes; d < 32; d <<= 1) {
 #pragma unroll
-    for (int m = 0; m < VN; ++m) sums[warp][lane][m] = acc[m];
-    __syncthreads();
-    if (warp == 0 && j < a.ncv) {
-      for (int k = 1; k < kWarps; ++k) {
-#pragma unroll
-        for (int m = 0; m < VN; ++m) acc[m] += sums[k][lane][m];
+      for (int m = 0; m < VN; ++m) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], d);
+    }
+  };
+  chain_enter();
+  const uint32_t chains = a.chains[0];
+  const int64_t windows = (a.count + a.window - 1) / a.window;
+  for (uint32_t item0 = blockIdx.x * kWarps; item0 < chains; item0 += gridDim.x * kWarps) {
+    const uint32_t item = item0 + warp;
+    int64_t w = 0, n = 0;
+    uint32_t cur = 0;
+    if (item < chains) {
+      w = a.chains[1 + item];
+      cur = a.items[(w + 1) * a.window - 1].x;
+      // the first window behind w that does not begin with this row: the next 32, then
+      // 32 probes a step; lo begins with it, the answer is in (lo, hi]
+      int64_t lo = w + 1, hi = windows, step = 1;
+      while (hi - lo > 1) {
+        const int64_t at = lo + step * (lane + 1);
+        const bool same = at < hi && a.items[at * a.window].x == cur;
+        const int found = __popc(__ballot_sync(0xffffffffu, same));  // a prefix of the lanes
+        const int64_t next = lo + step * (found + 1);
+        lo += step * found;
+        if (found < 32 && next < hi) hi = next;
+        step = (hi - lo + 31) / 32;
       }
-      store_row<T, VN>(out + (int64_t)cur * a.dim, j, a.dim, acc, a.scale);
+      n = hi - w;  // partial sums
+    }
+    const bool lengthy = n > (int64_t)kLongChain * parts;
+    if (n > 0 && !lengthy) {
+      float acc[VN];
+#pragma unroll
+      for (int m = 0; m < VN; ++m) acc[m] = 0.0f;
+      if (on) add(acc, w, n * mine / parts, n * (mine + 1) / parts);
+      over_groups(acc);
+      if (on && mine == 0) store_row<T, VN>(out + (int64_t)cur * a.dim, j, a.dim, acc, a.scale);
+    }
+    __syncthreads();
+    if (lane == 0) {
+      long_w[warp] = (uint32_t)w;
+      long_n[warp] = lengthy ? (uint32_t)n : 0;
+    }
+    __syncthreads();
+    for (int c = 0; c < kWarps; ++c) {
+      if (long_n[c] == 0) continue;
+      const int64_t lw = long_w[c], ln = long_n[c];
+      const int all = kWarps * parts, me = warp * parts + mine;
+      float acc[VN];
+#pragma unroll
+      for (int m = 0; m < VN; ++m) acc[m] = 0.0f;
+      if (on) add(acc, lw, ln * me / all, ln * (me + 1) / all);
+      over_groups(acc);
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < VN; ++m) sums[warp][lane][m] = acc[m];
+      __syncthreads();
+      if (warp == 0 && mine == 0 && on) {
+        for (int k = 1; k < kWarps; ++k) {
+#pragma unroll
+          for (int m = 0; m < VN; ++m) acc[m] += sums[k][lane][m];
+        }
+        const uint32_t row = a.items[(lw + 1) * a.window - 1].x;
+        store_row<T, VN>(out + (int64_t)row * a.dim, j, a.dim, acc, a.scale);
+      }
     }
   }
 }
@@ -618,9 +790,8 @@ static int window_of(int64_t count, int64_t dim) {
 }
 
 struct LookWs {
-  uint2* items;
-  uint32_t *k1, *v1, *k2, *v2, *chains;
-  int64_t *hist, *stmp;
+  uint2 *items, *other;
+  uint32_t *chains, *counts, *totals;
   float* part;
 };
 
@@ -629,14 +800,12 @@ static void carve_look(Carver& cv, LookWs& w, int64_t count, int64_t dim) {
   const int64_t windows = ceil_div64(e, window_of(e, dim));
   w.chains = cv.take<uint32_t>(windows + 1);
   w.items = cv.take<uint2>(e);
-  w.k1 = w.v1 = w.k2 = w.v2 = nullptr;
-  w.hist = w.stmp = nullptr;
+  w.other = nullptr;
+  w.counts = w.totals = nullptr;
   if (e > kSortMost) {
-    w.k1 = cv.take<uint32_t>(e); w.v1 = cv.take<uint32_t>(e);
-    w.k2 = cv.take<uint32_t>(e); w.v2 = cv.take<uint32_t>(e);
-    const int64_t nh = radix_hist_elems(1, e);
-    w.hist = cv.take<int64_t>(nh);
-    w.stmp = cv.take<int64_t>(scan_tmp_elems(nh));
+    w.other = cv.take<uint2>(e);
+    w.counts = cv.take<uint32_t>(kDigits * ceil_div64(e, kTile));
+    w.totals = cv.take<uint32_t>(kDigits);
   }
   w.part = cv.take<float>((size_t)(2 * windows * (dim + 16)));  // a row cut by its boundaries
 }
@@ -664,10 +833,12 @@ static int launch_sums(SumArgs a, const void* g, void* out, cudaStream_t st) {
         a, (const T*)g, (T*)out);
   SINKSLOT_CHECK_LAUNCH();
   if (windows == 1) return kOk;  // nothing crosses
+  int lanes = 1;
+  while (lanes < 32 && lanes < a.ncv) lanes *= 2;
   int64_t x = ceil_div64(6 * num_sms(), groups);
-  if (x > windows) x = windows;
+  if (x > ceil_div64(windows, kLookThreads / 32)) x = ceil_div64(windows, kLookThreads / 32);
   SINKSLOT_CUDA_TRY(launch_chained(lookup_join_kernel<T, VN>, dim3((unsigned)x, (unsigned)groups),
-                                   dim3(kLookThreads), 0, st, a, (T*)out));
+                                   dim3(kLookThreads), 0, st, a, lanes, (T*)out));
   return kOk;
 }
 
@@ -689,15 +860,20 @@ static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_
   if (count > kSortMost) {
     SINKSLOT_CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)out_bytes, st));
     SINKSLOT_CUDA_TRY(cudaMemsetAsync(w.chains, 0, sizeof(uint32_t), st));
-    lookup_key_kernel<<<(unsigned)ceil_div64(count, 256), 256, 0, st>>>(index, index_bytes, count,
-                                                                       rows, padding, w.k1);
-    SINKSLOT_CHECK_LAUNCH();
-    bool alt = false;
-    SINKSLOT_TRY(radix_sort_pairs<uint32_t>(w.k1, w.v1, w.k2, w.v2, true, 1, count, bits, w.hist,
-                                            w.stmp, &alt, st));
-    lookup_zip_kernel<<<(unsigned)ceil_div64(count, 256), 256, 0, st>>>(
-        alt ? w.k2 : w.k1, alt ? w.v2 : w.v1, count, w.items);
-    SINKSLOT_CHECK_LAUNCH();
+    const int tiles = (int)ceil_div64(count, kTile);
+    const int passes = (bits + kDigitBits - 1) / kDigitBits;
+    TileSource a = {index, index_bytes, count, rows, padding, nullptr, 0};
+    for (int k = 0; k < passes; ++k, a.shift += kDigitBits) {
+      uint2* to = (passes - k) & 1 ? w.items : w.other;  // the last pass fills w.items
+      SINKSLOT_CUDA_TRY(launch_chained(tile_count_kernel, dim3((unsigned)tiles),
+                                       dim3(kTileThreads), 0, st, a, tiles, w.counts));
+      SINKSLOT_CUDA_TRY(launch_chained(tile_scan_kernel, dim3(kDigits / 8), dim3(256), 0, st,
+                                       w.counts, tiles, w.totals));
+      SINKSLOT_CUDA_TRY(launch_chained(tile_scatter_kernel, dim3((unsigned)tiles),
+                                       dim3(kTileThreads), 0, st, a, tiles,
+                                       (const uint32_t*)w.counts, (const uint32_t*)w.totals, to));
+      a.items = to;
+    }
     return kOk;
   }
   int split = 1;
