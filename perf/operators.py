@@ -376,7 +376,8 @@ def _own_preference(s):
             tokens = torch.where(mask, tokens, IGNORE)
         logp = token_logprobs(leaf, tokens, ignore_index=IGNORE)
     r = preference_loss(logp, s["offsets"], ref_logp=s["ref"], mask=mask, beta=0.1,
-                        label_smoothing=c["smoothing"], kind=c["kind"], normalize=c["normalize"])
+                        label_smoothing=c["smoothing"] if c["kind"] == "sigmoid" else 0.0,
+                        kind=c["kind"], normalize=c["normalize"])
     grad, = torch.autograd.grad(r.loss, [leaf], s["outer"])
     return {"loss": r.loss.detach(), "chosen": r.chosen_rewards, "rejected": r.rejected_rewards,
             "grad": grad}
