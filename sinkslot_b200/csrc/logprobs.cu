@@ -34,7 +34,7 @@ __device__ __forceinline__ void write_row(const Online& o, const T* p, int64_t v
   logp[row] = token_logp(o, p, vocab, tok, inv_temp);
   if (kEnt)
     entropy[row] =
-        o.s == 0.0f ? 0.0f : (float)(log((double)o.s) - inv_temp * (double)(o.w / o.s));
+        o.s == 0.0f ? 0.0f : (float)(log_sum(o.s) - inv_temp * (double)(o.w / o.s));
   stats[row] = make_float2(o.m, o.s);
 }
 

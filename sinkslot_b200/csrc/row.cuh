@@ -17,7 +17,6 @@ constexpr int kRowUnroll = 4;  // 16-byte loads in flight per thread
 // exponent) would have the same sign for a whole row: at differences of -10 to -20 it
 // shifted each log-probability by 1.5e-7, which does not average out over a
 // sequence (measured on 2000-token sums).
-// hi is the next float below the value, so that lo > 0 and -inf times either is -inf.
 __device__ __forceinline__ float exp_scaled(float d, Scale2 c) {
   return exp2_fast(fmaf(d, c.hi, d * c.lo));
 }
@@ -33,7 +32,7 @@ struct Online {
 template <bool kEnt>
 __device__ __forceinline__ void rebase(Online& o, float m2, Scale2 c) {
   const float d = o.m - m2;  // <= 0
-  const float a = expf(d * c.inv);
+  const float a = expf(fmaf(d, c.inv, d * c.inv_lo));
   if (kEnt) o.w = a > 0.0f ? (o.w + o.s * d) * a : 0.0f;  // d may be -inf, or near it, where a is 0
   o.s *= a;
   o.m = m2;
@@ -94,13 +93,18 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64
                     : (int64_t) static_cast<const int32_t*>(tokens)[r];
 }
 
-// In fp64 until the result is rounded: logf's error has a mean of its own, 1e-7 of
-// a log-probability (measured), which a sequence's sum would keep.
+// ln s in fp64: logf's error has a mean of its own, 1e-7 of a log-probability
+// (measured), which a sequence's sum would keep.  So has the sum's: it comes out low
+// by 2.0e-8 to 3.5e-8 of its value (64 to 131072 terms of the three types; exp2_fast
+// is low by 5e-8 on average in every octave but the first), the largest term, 1, apart.
+__device__ __forceinline__ double log_sum(float s) {
+  return log((double)s) + 2.7e-8 * (1.0 - 1.0 / (double)s);
+}
 __device__ __forceinline__ float token_logp_of(const Online& o, float at_tok, bool inside,
                                                double inv_temp) {
   if (!inside) return __int_as_float(0x7fc00000);
   if (o.s == 0.0f) return -INFINITY;
-  return (float)((double)(at_tok - o.m) * inv_temp - log((double)o.s));
+  return (float)((double)(at_tok - o.m) * inv_temp - log_sum(o.s));
 }
 template <typename T>
 __device__ __forceinline__ float token_logp(const Online& o, const T* p, int64_t vocab,
@@ -275,11 +279,17 @@ __device__ __forceinline__ float inverse_sum(float s) {
   return s > 0.0f ? 1.0f / s : (s == 0.0f ? 0.0f : s);
 }
 
+// hi is below v, and v - hi is lo > 0: -inf times either is -inf.
+inline void halves(double v, float& hi, float& lo) {
+  hi = (float)v;
+  if ((double)hi >= v) hi = std::nextafterf(hi, 0.0f);
+  lo = (float)(v - (double)hi);
+}
 inline Scale2 scale2(double inv_temp) {
-  const double c = inv_temp * 1.4426950408889634;
-  float hi = (float)c;
-  if ((double)hi >= c) hi = std::nextafterf(hi, 0.0f);
-  return {hi, (float)(c - (double)hi), (float)inv_temp};
+  Scale2 c;
+  halves(inv_temp * 1.4426950408889634, c.hi, c.lo);
+  halves(inv_temp, c.inv, c.inv_lo);
+  return c;
 }
 
 }  // namespace sinkslot
