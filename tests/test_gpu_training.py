@@ -703,3 +703,63 @@ def test_offsets_that_lie_stay_in_bounds(sk):
         p = sk.preference_loss(logp, offsets)
         torch.autograd.grad(p.loss, [logp])
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ sizes past 32 bits
+def test_logits_of_more_than_2_to_the_31_elements(sk):
+    """The last rows of 16400 x 131072 logits, through the log-probabilities' own kernels and the
+    policy loss's."""
+    t, vocab = 16400, 131072
+    assert t * vocab > 2 ** 31
+    gen = _gen(81)
+    z = torch.empty(t, vocab, device="cuda", dtype=torch.bfloat16)
+    z.normal_(0.0, 2.0, generator=gen)
+    tokens = torch.randint(0, vocab, (t,), generator=gen, device="cuda")
+    z.requires_grad_()
+    g = torch.randn(t, generator=gen, device="cuda")
+    lp = sk.token_logprobs(z, tokens)
+    grad, = torch.autograd.grad(lp, [z], g)
+    for rows in (slice(0, 3), slice(t - 3, t)):
+        zd, tk = z.detach()[rows], tokens[rows]
+        want, *_ = ref.logprobs64(zd, tk)
+        _close(lp.detach()[rows], want, ref.logp_tolerance(zd, tk, 1.0, vocab), "logp")
+        wgrad = ref.logprobs_grad64(zd, tk, g[rows])
+        _close(grad[rows], wgrad, _grad_tolerance(zd, tk, g[rows], None, 1.0, wgrad, z.dtype),
+               "grad")
+    del grad
+    old = lp.detach() + 0.05
+    r = sk.policy_loss_from_logits(z, tokens, old, g, grad_scale=float(t))
+    grad, = torch.autograd.grad(r.loss, [z], torch.tensor(float(t), device="cuda"))
+    # (the two ways of summing a row are each within the tolerance of the same value)
+    _close(r.logp, lp.detach(), 2 * ref.logp_tolerance(z.detach()[:8], tokens[:8], 1.0, vocab).max()
+           + 8 * EPS32 * lp.detach().double().abs(), "logp, two ways")
+    for rows in (slice(0, 3), slice(t - 3, t)):
+        zd, tk = z.detach()[rows], tokens[rows]
+        ltol = float(ref.logp_tolerance(zd, tk, 1.0, vocab).max())
+        coef = -torch.exp(lp.detach()[rows].double() - old[rows].double()) * g[rows].double()
+        coef = torch.where((g[rows] < 0) & (lp.detach()[rows] - old[rows] < math.log(0.8)),
+                           torch.zeros_like(coef), coef)
+        wgrad = ref.logprobs_grad64(zd, tk, coef)
+        _close(grad[rows], wgrad, _grad_tolerance(zd, tk, coef, None, 1.0, wgrad, z.dtype)
+               + wgrad.abs() * (4 * ltol + 32 * EPS32), "policy grad")
+
+
+def test_table_of_more_than_2_to_the_31_elements(sk):
+    rows, dim = 600000, 4096
+    assert rows * dim > 2 ** 31
+    gen = _gen(82)
+    table = torch.empty(rows, dim, device="cuda", dtype=torch.float16)
+    table.normal_(0.0, 1.0, generator=gen)
+    table.requires_grad_()
+    index = torch.tensor([rows - 1, 0, rows - 1, 1, rows - 2, 555555], device="cuda")
+    out = sk.embedding_lookup(table, index, scale=0.5)
+    assert torch.equal(out, (table.detach()[index].float() * 0.5).half())
+    g = torch.randn(6, dim, generator=gen, device="cuda").half()
+    grad, = torch.autograd.grad(out, [table], g)
+    want = torch.zeros(4, dim, dtype=torch.float64, device="cuda")
+    for k, row in enumerate([rows - 1, 0, rows - 2, 555555]):
+        want[k] = 0.5 * g[index == row].double().sum(0)
+    got = grad[torch.tensor([rows - 1, 0, rows - 2, 555555], device="cuda")]
+    # two addends at most, of a few units: one float32 addition, then the type's rounding
+    _close(got, want, half_step(torch.float16) * want.abs() + 8 * EPS32 + tiny(torch.float16), "rows")
+    assert int((grad != 0).any(1).sum()) == 5
