@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_row_kernel(LogitRows r, i
 // Rows of at most this many bytes go to a warp each.
 constexpr int64_t kWarpRowBytes = 4096;
 
-static int check_rows(const LogitRows& r) {
+int check_rows(const LogitRows& r) {
   SINKSLOT_REQUIRE(dtype_ok(r.dtype), "token_logprobs: dtype must be 0, 1 or 2");
   SINKSLOT_REQUIRE(r.rows >= 0 && r.vocab >= 1 && r.stride >= 0, "token_logprobs: bad sizes");
   SINKSLOT_REQUIRE(r.vocab <= int64_t(1) << 30, "token_logprobs: more than 2^30 tokens to choose");

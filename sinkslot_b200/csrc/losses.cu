@@ -430,7 +430,12 @@ int policy_loss_logits(const LogitRows& r, const Packed& p, const PolicyTerms& t
                        float* values, float* logp, void* dz, int64_t dz_stride, void* ws,
                        size_t ws_bytes, cudaStream_t st) {
   SINKSLOT_REQUIRE(p.tokens == r.rows, "policy_loss_from_logits: bad sizes");
+  SINKSLOT_TRY(check_rows(r));
   SINKSLOT_TRY(check_packed(p));
+  SINKSLOT_REQUIRE(values && (r.rows == 0 || (logp && t.old_logp && t.adv)),
+                   "policy_loss_from_logits: null argument");
+  SINKSLOT_REQUIRE(!dz || dz_stride >= r.vocab || r.rows <= 1,
+                   "policy_loss_from_logits: rows of the gradient overlap");
   Carver cv(ws, ws_bytes);
   float2* stats = cv.take<float2>((size_t)(r.rows > 0 ? r.rows : 1));
   float* coef = cv.take<float>((size_t)(r.rows > 0 ? r.rows : 1));

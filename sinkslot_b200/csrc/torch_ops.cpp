@@ -613,8 +613,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_from_logits(
   TORCH_CHECK_VALUE(logits.dim() == 2, name, ": logits must be (tokens, vocab), got ",
                     logits.sizes());
   check_logits(name, logits, tokens, temperature);
-  TORCH_CHECK_VALUE(std::isfinite(grad_scale) && grad_scale != 0.0, name,
-                    ": grad_scale must be finite and not 0, got ", grad_scale);
+  TORCH_CHECK_VALUE(std::isnormal((float)grad_scale), name,
+                    ": grad_scale must be a normal float32, got ", grad_scale);
   const PolicyInputs in = check_policy(name, tokens, old_logp, advantages, ref_logp, mask, offsets,
                                        clip_low, clip_high, kl_coef, kl, average);
   const Tensor z = unit_rows(logits), flat = tokens.contiguous();

@@ -41,6 +41,7 @@ struct LogitRows {
   double inv_temp = 1.0;
   Scale2 scale;  // set by token_logprobs
 };
+int check_rows(const LogitRows& r);
 int token_logprobs(const LogitRows& r, float* logp, float* entropy, float2* stats,
                    cudaStream_t st);
 // g, g_entropy: outer gradients (nullable), their strides in elements (0: one

@@ -136,6 +136,15 @@ def _f32(like, *shape):
     return like.new_empty(shape, dtype=torch.float32)
 
 
+def _grad_like(z):
+    """Rows as far apart as the logits' own, contiguous where those overlap."""
+    rows, vocab = z.shape
+    stride = z.stride(0)
+    if rows <= 1 or stride < vocab:
+        stride = vocab
+    return torch.empty_strided((rows, vocab), (stride, 1), dtype=z.dtype, device=z.device)
+
+
 # Output shapes of the training operators that launch (the functions above them,
 # embedding_lookup, logprobs, policy, policy_from_logits and preference, are
 # made of these).
@@ -146,11 +155,12 @@ _TRAINING_FAKES = {
         _f32(z, z.shape[0]), _f32(z, z.shape[0] if entropy else 0), _f32(z, z.shape[0], 2)),
     "token_logprobs_grad":
         lambda z, tokens, stats, entropy, g, g_entropy, temperature, ignore_index:
-        z.new_empty(z.shape),
+        _grad_like(z),
     "policy_loss": lambda logp, *a: (_f32(logp, 4), _f32(logp, logp.shape[0] if a[-1] else 0)),
     "scale_tokens": lambda coef, values, g: torch.empty_like(coef),
     "policy_loss_logits": lambda z, *a: (
-        _f32(z, 4), _f32(z, z.shape[0]), z.new_empty((z.shape[0] if a[-1] else 0, z.shape[1]))),
+        _f32(z, 4), _f32(z, z.shape[0]),
+        _grad_like(z) if a[-1] else z.new_empty((0, z.shape[1]))),
     "scale_rows_": lambda grad, g, grad_scale: None,
     "preference_loss": lambda logp, offsets, *a: (
         _f32(logp), _f32(logp, offsets.shape[0] - 1), _f32(logp, offsets.shape[0] - 1)),

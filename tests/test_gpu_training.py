@@ -705,6 +705,86 @@ def test_offsets_that_lie_stay_in_bounds(sk):
     torch.cuda.synchronize()
 
 
+def test_second_derivatives_are_refused(sk):
+    """create_graph gives the first derivative; differentiating it again is an error."""
+    gen = _gen(71)
+    table = torch.randn(20, 8, generator=gen, device="cuda", requires_grad=True)
+    z = torch.randn(6, 300, generator=gen, device="cuda", requires_grad=True)
+    lp = -torch.rand(12, generator=gen, device="cuda")
+    lp.requires_grad_()
+    ids = torch.randint(0, 20, (6,), generator=gen, device="cuda")
+    old = torch.full((6,), -5.0, device="cuda")
+    offsets = torch.tensor([0, 5, 12], device="cuda")
+    for make, leaf in [
+            (lambda: sk.embedding_lookup(table, ids).square().sum(), table),
+            (lambda: sk.token_logprobs(z, ids).square().sum(), z),
+            (lambda: sk.policy_loss(lp, lp.detach(), torch.ones(12, device="cuda")).loss.square(), lp),
+            (lambda: sk.policy_loss_from_logits(z, ids, old, old).loss, z),
+            (lambda: sk.preference_loss(lp, offsets).loss.square(), lp)]:
+        plain, = torch.autograd.grad(make(), [leaf])
+        first, = torch.autograd.grad(make(), [leaf], create_graph=True)
+        assert torch.equal(plain, first) and first.requires_grad
+        # (where the loss is linear, torch finds no way from the derivative back to the leaf)
+        with pytest.raises(RuntimeError, match="second derivative|not have been used"):
+            torch.autograd.grad(first.sum(), [leaf])
+
+
+def test_policy_from_logits_without_rows(sk):
+    z = torch.empty(0, 40, device="cuda", dtype=torch.float16, requires_grad=True)
+    none = torch.empty(0, device="cuda")
+    r = sk.policy_loss_from_logits(z, none.long(), none, torch.ones(2, device="cuda"),
+                                   offsets=torch.zeros(3, dtype=torch.int64, device="cuda"))
+    grad, = torch.autograd.grad(r.loss, [z])
+    assert float(r.loss.detach()) == 0.0 and grad.shape == (0, 40) and r.logp.shape == (0,)
+
+
+def test_captured_large_paths(sk):
+    """What only large sizes take, captured and replayed on other inputs: zeros beside the sort, the
+    tile sort, one pass over rows larger than L2."""
+    gen = _gen(91)
+
+    def inputs():
+        return {
+            "wide": torch.randn(9000, 2048, generator=gen, device="cuda").bfloat16(),
+            "ids": torch.randint(0, 9000, (700,), generator=gen, device="cuda"),
+            "narrow": torch.randn(3000, 5, generator=gen, device="cuda"),
+            "many": torch.randint(0, 3000, (120000,), generator=gen, device="cuda"),
+            "z": torch.randn(2200, 32768, generator=gen, device="cuda").bfloat16(),
+            "tokens": torch.randint(0, 32768, (2200,), generator=gen, device="cuda"),
+            "old": torch.full((2200,), -11.0, device="cuda"),
+            "adv": torch.randn(2200, generator=gen, device="cuda"),
+            "ga": torch.randn(700, 2048, generator=gen, device="cuda").bfloat16(),
+            "gb": torch.randn(120000, 5, generator=gen, device="cuda")}
+
+    def step(s):
+        a = torch.autograd.grad(sk.embedding_lookup(s["wide"], s["ids"], 3.0), [s["wide"]], s["ga"])
+        b = torch.autograd.grad(sk.embedding_lookup(s["narrow"], s["many"]), [s["narrow"]], s["gb"])
+        r = sk.policy_loss_from_logits(s["z"], s["tokens"], s["old"], s["adv"])
+        c = torch.autograd.grad(r.loss, [s["z"]])
+        return [*a, *b, r.loss.detach(), r.logp, *c]
+
+    s = inputs()
+    for k in ("wide", "narrow", "z"):
+        s[k].requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(s)
+    fresh = inputs()
+    with torch.no_grad():
+        for k, v in s.items():
+            v.copy_(fresh[k])
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, step(s)):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------ sizes past 32 bits
 def test_logits_of_more_than_2_to_the_31_elements(sk):
     """The last rows of 16400 x 131072 logits, through the log-probabilities' own kernels and the

@@ -105,6 +105,8 @@ def test_policy_refusals(fake):
             (lambda: sk.policy_loss_from_logits(_cuda(20, 9), _ids(19), old, adv, **ok), "tokens"),
             (lambda: sk.policy_loss_from_logits(_cuda(20, 9), _ids(20), old, adv, grad_scale=0.0,
                                                 **ok), "grad_scale"),
+            (lambda: sk.policy_loss_from_logits(_cuda(20, 9), _ids(20), old, adv, grad_scale=1e200,
+                                                **ok), "grad_scale"),
     ]:
         with pytest.raises(ValueError, match=match):
             bad()
@@ -161,6 +163,12 @@ def test_c_entries_check_their_arguments():
                                          None)),
             ("sinkslot_policy_loss", (None, None, None, None, 0, None, None, 8, 2, 5, 0.2, 0.2, 0.0,
                                       3, 0, None, None, None, 0, None)),
+            ("sinkslot_policy_loss_logits", (None, 2, 9, 3, 9, None, 8, 1.0, None, None, None, 0,
+                                             None, None, 8, 1, 0.2, 0.2, 0.0, 3, 0, 1.0, None, None,
+                                             None, 0, None, 0, None)),
+            ("sinkslot_policy_loss_logits", (None, 5, 9, 0, 9, None, 8, 1.0, None, None, None, 0,
+                                             None, None, 8, 1, 0.2, 0.2, 0.0, 3, 0, 1.0, None, None,
+                                             None, 0, None, 0, None)),
             ("sinkslot_preference_loss", (None, None, None, None, 8, 3, 5, 0.1, 0.0, 0, 0, None,
                                           None, None, None, 0, None))]:
         with pytest.raises(ValueError):
