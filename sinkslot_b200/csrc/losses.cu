@@ -26,6 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int kLossThreads = 512;
 constexpr int kLossWarps = kLossThreads / 32;
 constexpr int kLossSplit = 8;
+constexpr int kAtOnce = 4;  // tokens that a thread loads together
 
 struct Sums {
   double a, b, c;
@@ -101,14 +102,11 @@ __device__ __forceinline__ void zero_outside(const Packed& p, int64_t seq, int64
     for (int64_t t = offset_at(p, p.count) + at; t < p.tokens; t += step) out[t] = 0.0f;
 }
 
-// Per sequence: {loss, kl, clipped, counted}.
-__global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, PolicyTerms t,
-                                                                  PolicyEdges e, int split,
-                                                                  double4* __restrict__ part,
-                                                                  float* __restrict__ coef) {
-  __shared__ ClusterSum sh;
-  const int64_t seq = blockIdx.x / (unsigned)split;
-  const int rank = (int)(blockIdx.x % (unsigned)split);
+// One sequence, by `split` CTAs of a cluster: part = {loss, kl, clipped, counted}.
+__device__ __forceinline__ void policy_seq(const Packed& p, const PolicyTerms& t,
+                                           const PolicyEdges& e, int64_t seq, int rank, int split,
+                                           ClusterSum& sh, double4* part,
+                                           float* __restrict__ coef) {
   const int64_t at = (int64_t)rank * kLossThreads + threadIdx.x;
   const int64_t step = (int64_t)split * kLossThreads;
   int64_t lo, hi;
@@ -118,6 +116,7 @@ __global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, Poli
     double n = (double)(hi - lo);
     if (p.mask) {
       int64_t k = 0;
+#pragma unroll 4
       for (int64_t i = lo + at; i < hi; i += step) k += p.mask[i] != 0;
       n = cluster_sums({(double)k, 0.0, 0.0}, sh, 0, rank, split).a;
     }
@@ -126,16 +125,40 @@ __global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, Poli
   const float finv = (float)inv;
   Sums s = {0.0, 0.0, 0.0};
   int64_t n = 0;
-  for (int64_t i = lo + at; i < hi; i += step) {
-    float cf = 0.0f;
-    if (!p.mask || p.mask[i]) {
-      const TokenTerm o = policy_term(t, e, t.logp[i], i, seq);
-      s.a += (double)o.loss;
-      s.b += (double)o.kl;
-      n += 1 + ((int64_t)o.clipped << 32);
-      cf = o.coef * finv;
+  const float seq_adv = t.adv_per_token || lo >= hi ? 0.0f : t.adv[seq];
+  for (int64_t i = lo + at; i < hi; i += kAtOnce * step) {
+    // what the tokens need is loaded for all of them at once, masked ones too (their
+    // values are not looked at)
+    bool on[kAtOnce];
+    float logp[kAtOnce], old_logp[kAtOnce], ref_logp[kAtOnce], adv[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t j = i + k * step;
+      on[k] = j < hi;
+      logp[k] = old_logp[k] = ref_logp[k] = 0.0f;
+      adv[k] = seq_adv;
+      if (j < hi) {
+        if (p.mask) on[k] = p.mask[j] != 0;
+        logp[k] = t.logp[j];
+        old_logp[k] = t.old_logp[j];
+        if (t.ref_logp) ref_logp[k] = t.ref_logp[j];
+        if (t.adv_per_token) adv[k] = t.adv[j];
+      }
     }
-    if (coef) coef[i] = cf;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t j = i + k * step;
+      if (j >= hi) break;
+      float cf = 0.0f;
+      if (on[k]) {
+        const TokenTerm o = policy_term(t, e, logp[k], old_logp[k], ref_logp[k], adv[k]);
+        s.a += (double)o.loss;
+        s.b += (double)o.kl;
+        n += 1 + ((int64_t)o.clipped << 32);
+        cf = o.coef * finv;
+      }
+      if (coef) coef[j] = cf;
+    }
   }
   zero_outside(p, seq, at, step, coef);
   // counts of counted and of clipped tokens, both under 2^32, apart in fp64
@@ -143,6 +166,15 @@ __global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, Poli
   const Sums f = cluster_sums(s, sh, 1, rank, split);
   const Sums k = cluster_sums({(double)(n >> 32), 0.0, 0.0}, sh, 0, rank, split);
   if (rank == 0 && threadIdx.x == 0) part[seq] = make_double4(f.a * inv, f.b * inv, k.a, f.c);
+}
+
+__global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, PolicyTerms t,
+                                                                  PolicyEdges e, int split,
+                                                                  double4* __restrict__ part,
+                                                                  float* __restrict__ coef) {
+  __shared__ ClusterSum sh;
+  policy_seq(p, t, e, blockIdx.x / (unsigned)split, (int)(blockIdx.x % (unsigned)split), split, sh,
+             part, coef);
   chain_release();
 }
 
@@ -151,11 +183,9 @@ __device__ __forceinline__ Sums cta_sums(Sums v, ClusterSum& sh, int turn) {
   return cluster_sums(v, sh, turn, 0, 1);
 }
 
-__global__ void __launch_bounds__(kLossThreads) policy_end_kernel(const double4* __restrict__ part,
-                                                                  int64_t count, int by_sequence,
-                                                                  float* __restrict__ values) {
-  __shared__ ClusterSum sh;
-  chain_enter();
+// All sequences, by one CTA.
+__device__ __forceinline__ void policy_end(const double4* part, int64_t count, int by_sequence,
+                                           ClusterSum& sh, float* __restrict__ values) {
   Sums s = {0.0, 0.0, 0.0}, k = {0.0, 0.0, 0.0};
   for (int64_t i = threadIdx.x; i < count; i += kLossThreads) {
     const double4 v = part[i];
@@ -175,6 +205,35 @@ __global__ void __launch_bounds__(kLossThreads) policy_end_kernel(const double4*
     values[2] = k.a > 0.0 ? (float)(s.c / k.a) : 0.0f;
     values[3] = (float)norm;
   }
+}
+
+__global__ void __launch_bounds__(kLossThreads) policy_end_kernel(const double4* __restrict__ part,
+                                                                  int64_t count, int by_sequence,
+                                                                  float* __restrict__ values) {
+  __shared__ ClusterSum sh;
+  chain_enter();
+  policy_end(part, count, by_sequence, sh, values);
+}
+
+// Both in one launch, for few tokens: one cluster, its CTAs taking sequences in turn.
+__global__ void __launch_bounds__(kLossThreads) policy_small_kernel(Packed p, PolicyTerms t,
+                                                                    PolicyEdges e, double4* part,
+                                                                    float* __restrict__ coef,
+                                                                    float* __restrict__ values) {
+  __shared__ ClusterSum sh;
+  for (int64_t seq = blockIdx.x; seq < p.count; seq += gridDim.x)
+    policy_seq(p, t, e, seq, 0, 1, sh, part, coef);
+  cg::this_cluster().sync();
+  if (blockIdx.x == 0) policy_end(part, p.count, t.sequence_average, sh, values);
+}
+
+// One launch where that costs no time on the GPU, a sequence for each CTA: the host's
+// is what small calls wait for (a launch is 3 of 70 us, forward and backward).
+static bool small_loss(const Packed& p) { return p.tokens <= 16384 && p.count <= kLossSplit; }
+static int small_ctas(const Packed& p) {
+  int ctas = 1;
+  while (ctas < kLossSplit && ctas < p.count) ctas *= 2;
+  return ctas;
 }
 
 // CTAs for each sequence: a cluster of 8 while the sequences do not fill the
@@ -228,6 +287,12 @@ int policy_loss(const Packed& p, const PolicyTerms& t, float* values, float* coe
     return kWorkspaceTooSmall;
   }
   double4* part = static_cast<double4*>(ws);
+  if (small_loss(p)) {
+    const int ctas = small_ctas(p);
+    SINKSLOT_CUDA_TRY(launch_cluster(policy_small_kernel, 1, ctas, kLossThreads, st, p, t,
+                                     policy_edges(t), part, coef, values));
+    return kOk;
+  }
   const int split = loss_split(p);
   SINKSLOT_CUDA_TRY(launch_cluster(policy_seq_kernel, p.count, split, kLossThreads, st, p, t,
                                    policy_edges(t), split, part, coef));
@@ -239,34 +304,55 @@ int policy_loss(const Packed& p, const PolicyTerms& t, float* values, float* coe
 // --------------------------------------------------------------------------
 // Preference loss
 // --------------------------------------------------------------------------
-__global__ void __launch_bounds__(kLossThreads) preference_seq_kernel(
-    Packed p, const float* __restrict__ logp, const float* __restrict__ ref, int split,
-    double2* __restrict__ part) {
-  __shared__ ClusterSum sh;
-  const int64_t seq = blockIdx.x / (unsigned)split;
-  const int rank = (int)(blockIdx.x % (unsigned)split);
+__device__ __forceinline__ void preference_seq(const Packed& p, const float* __restrict__ logp,
+                                               const float* __restrict__ ref, int64_t seq,
+                                               int rank, int split, ClusterSum& sh,
+                                               double2* part) {
   int64_t lo, hi;
   bounds(p, seq, lo, hi);
   Sums s = {0.0, 0.0, 0.0};
   int64_t n = 0;
-  for (int64_t i = lo + (int64_t)rank * kLossThreads + threadIdx.x; i < hi;
-       i += (int64_t)split * kLossThreads) {
-    if (p.mask && !p.mask[i]) continue;
-    s.a += (double)logp[i] - (ref ? (double)ref[i] : 0.0);
-    ++n;
+  const int64_t step = (int64_t)split * kLossThreads;
+  for (int64_t i = lo + (int64_t)rank * kLossThreads + threadIdx.x; i < hi; i += kAtOnce * step) {
+    bool on[kAtOnce];
+    float a[kAtOnce], b[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t j = i + k * step;
+      on[k] = j < hi;
+      a[k] = b[k] = 0.0f;
+      if (j < hi) {
+        if (p.mask) on[k] = p.mask[j] != 0;
+        a[k] = logp[j];
+        if (ref) b[k] = ref[j];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (on[k]) {
+        s.a += (double)a[k] - (double)b[k];
+        ++n;
+      }
   }
   s.b = (double)n;
   const Sums f = cluster_sums(s, sh, 0, rank, split);
   if (rank == 0 && threadIdx.x == 0) part[seq] = make_double2(f.a, f.b);
+}
+
+__global__ void __launch_bounds__(kLossThreads) preference_seq_kernel(
+    Packed p, const float* __restrict__ logp, const float* __restrict__ ref, int split,
+    double2* __restrict__ part) {
+  __shared__ ClusterSum sh;
+  preference_seq(p, logp, ref, blockIdx.x / (unsigned)split, (int)(blockIdx.x % (unsigned)split),
+                 split, sh, part);
   chain_release();
 }
 
-__global__ void __launch_bounds__(kLossThreads) preference_end_kernel(
-    const double2* __restrict__ part, int64_t pairs, double beta, double smoothing, int kind,
-    int normalize, float* __restrict__ loss, float* __restrict__ rewards,
-    float* __restrict__ slope) {
-  __shared__ ClusterSum sh;
-  chain_enter();
+__device__ __forceinline__ void preference_end(const double2* part, int64_t pairs, double beta,
+                                               double smoothing, int kind, int normalize,
+                                               ClusterSum& sh, float* __restrict__ loss,
+                                               float* __restrict__ rewards,
+                                               float* __restrict__ slope) {
   Sums s = {0.0, 0.0, 0.0};
   for (int64_t i = threadIdx.x; i < pairs; i += kLossThreads) {
     const double2 c = part[i], r = part[pairs + i];
@@ -303,6 +389,27 @@ __global__ void __launch_bounds__(kLossThreads) preference_end_kernel(
   if (threadIdx.x == 0) loss[0] = (float)(s.a / (double)pairs);
 }
 
+__global__ void __launch_bounds__(kLossThreads) preference_end_kernel(
+    const double2* __restrict__ part, int64_t pairs, double beta, double smoothing, int kind,
+    int normalize, float* __restrict__ loss, float* __restrict__ rewards,
+    float* __restrict__ slope) {
+  __shared__ ClusterSum sh;
+  chain_enter();
+  preference_end(part, pairs, beta, smoothing, kind, normalize, sh, loss, rewards, slope);
+}
+
+__global__ void __launch_bounds__(kLossThreads) preference_small_kernel(
+    Packed p, PreferenceTerms t, double2* part, float* __restrict__ loss,
+    float* __restrict__ rewards, float* __restrict__ slope) {
+  __shared__ ClusterSum sh;
+  for (int64_t seq = blockIdx.x; seq < p.count; seq += gridDim.x)
+    preference_seq(p, t.logp, t.ref_logp, seq, 0, 1, sh, part);
+  cg::this_cluster().sync();
+  if (blockIdx.x == 0)
+    preference_end(part, p.count / 2, t.beta, t.smoothing, t.kind, t.normalize, sh, loss, rewards,
+                   slope);
+}
+
 int preference_loss(const Packed& p, const PreferenceTerms& t, float* loss, float* rewards,
                     float* slope, void* ws, size_t ws_bytes, cudaStream_t st) {
   SINKSLOT_TRY(check_packed(p));
@@ -315,6 +422,12 @@ int preference_loss(const Packed& p, const PreferenceTerms& t, float* loss, floa
     return kWorkspaceTooSmall;
   }
   double2* part = static_cast<double2*>(ws);
+  if (small_loss(p)) {
+    const int ctas = small_ctas(p);
+    SINKSLOT_CUDA_TRY(launch_cluster(preference_small_kernel, 1, ctas, kLossThreads, st, p, t,
+                                     part, loss, rewards, slope));
+    return kOk;
+  }
   const int split = loss_split(p);
   SINKSLOT_CUDA_TRY(launch_cluster(preference_seq_kernel, p.count, split, kLossThreads, st, p,
                                    t.logp, t.ref_logp, split, part));
@@ -333,6 +446,7 @@ __global__ void __launch_bounds__(kLossThreads) preference_grad_kernel(
   int64_t lo, hi;
   bounds(p, seq, lo, hi);
   const float v = slope[seq] * g[0];
+#pragma unroll 4
   for (int64_t i = lo + at; i < hi; i += step) out[i] = !p.mask || p.mask[i] ? v : 0.0f;
   zero_outside(p, seq, at, step, out);
 }

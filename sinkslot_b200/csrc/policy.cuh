@@ -31,9 +31,9 @@ struct TokenTerm {
 
 // One token's loss, KL estimate and d loss / d logp.  The clip is decided on the
 // difference of the log-probabilities in fp64, which is exact.
-__device__ __forceinline__ TokenTerm policy_term_of(const PolicyTerms& t, const PolicyEdges& e,
-                                                    float logp, float old_logp, float ref_logp,
-                                                    float adv) {
+__device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
+                                                 float logp, float old_logp, float ref_logp,
+                                                 float adv) {
   TokenTerm o;
   const double d = (double)logp - (double)old_logp;
   const bool over = d > e.over, under = d < e.under;
@@ -63,12 +63,6 @@ __device__ __forceinline__ TokenTerm policy_term_of(const PolicyTerms& t, const 
     }
   }
   return o;
-}
-
-__device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
-                                                 float logp, int64_t at, int64_t seq) {
-  return policy_term_of(t, e, logp, t.old_logp[at], t.ref_logp ? t.ref_logp[at] : 0.0f,
-                        t.adv[t.adv_per_token ? at : seq]);
 }
 
 inline PolicyEdges policy_edges(const PolicyTerms& t) {

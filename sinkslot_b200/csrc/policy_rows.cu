@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kSweepThreads, kSweepCtas) policy_rows_kernel(
     const float lp = token_logp_of(o, zt, inside, r.inv_temp);
     if (rank == 0) logp[row] = lp;
     const float g = weight == 0.0f ? 0.0f
-                                   : policy_term_of(t, e, lp, old_logp, ref_logp, adv).coef *
+                                   : policy_term(t, e, lp, old_logp, ref_logp, adv).coef *
                                          weight * grad_scale * (float)r.inv_temp;
     RowCoef q = {};
     q.m = o.m;
