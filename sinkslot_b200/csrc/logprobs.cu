@@ -186,7 +186,8 @@ int token_logprobs(const LogitRows& rows, float* logp, float* entropy, float2* s
 template <typename T, bool kEnt>
 __global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogitRows r, LogitGrad g,
                                                                    int share) {
-  const int64_t row = blockIdx.x;
+  // from the last row on: the forward pass left the end of the logits in L2
+  const int64_t row = r.rows - 1 - (int64_t)blockIdx.x;
   const int64_t tok = token_at(r.tokens, r.token_bytes, row);
   const T* p = static_cast<const T*>(r.z) + row * r.stride;
   T* out = static_cast<T*>(g.dz) + row * g.dz_stride;
