@@ -244,8 +244,8 @@ static size_t sort_smem(int per) { return sizeof(SortShared) + (size_t)per * 16;
 
 __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     const void* __restrict__ index, int index_bytes, int count, int64_t rows, int64_t padding,
-    int per, int bits, uint2* __restrict__ items, uint32_t* __restrict__ chains, uint4* __restrict__ zeros, int64_t zero_vecs,
-    int64_t zero_tail) {
+    int per, int bits, uint2* __restrict__ items, uint32_t* __restrict__ chains,
+    uint4* __restrict__ zeros, int64_t zero_vecs, int64_t zero_tail) {
   cg::cluster_group cl = cg::this_cluster();
   const int split = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   chain_release();  // what fills the rest of the table waits for nothing here

@@ -70,10 +70,46 @@ Tensor grad_like(const Tensor& z) {
   return flat.as_strided({rows, vocab}, {stride, 1}, phase);
 }
 
+int64_t sequences(const optional<Tensor>& offsets) {
+  return offsets.has_value() ? offsets->numel() - 1 : 1;
+}
+int offset_bytes(const optional<Tensor>& offsets) {
+  return offsets.has_value() ? (int)offsets->element_size() : 8;
+}
+
+// What a launching operator takes for granted of its tensors (the functions above
+// them see to it; a direct call that does not is refused).
+void expect(const Tensor& t, at::ScalarType type, int64_t numel, const char* what) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == type && t.numel() == numel &&
+                        t.is_contiguous(),
+                    what, ": expected a contiguous CUDA tensor of ", numel, " ", type, ", got ",
+                    t.sizes(), " ", t.scalar_type());
+}
+void expect(const optional<Tensor>& t, at::ScalarType type, int64_t numel, const char* what) {
+  if (t.has_value()) expect(*t, type, numel, what);
+}
+void expect_index(const Tensor& t, int64_t numel, const char* what) {
+  expect(t, t.scalar_type() == at::kInt ? at::kInt : at::kLong, numel, what);
+}
+void expect_rows(const Tensor& t, const char* what) {
+  const auto d = t.scalar_type();
+  TORCH_CHECK_VALUE(t.is_cuda() && t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) &&
+                        (d == at::kFloat || d == at::kHalf || d == at::kBFloat16),
+                    what, ": expected rows of contiguous float32, float16 or bfloat16, got ",
+                    t.sizes(), " ", d);
+}
+void expect_offsets(const optional<Tensor>& offsets) {
+  if (!offsets.has_value()) return;
+  TORCH_CHECK_VALUE(offsets->numel() >= 2, "offsets: expected two values or more");
+  expect_index(*offsets, offsets->numel(), "offsets");
+}
+
 // ---------------------------------------------------------------------------
 // Operators that launch
 // ---------------------------------------------------------------------------
 Tensor lookup(const Tensor& table, const Tensor& index, double scale) {
+  expect_rows(table, "table");
+  expect_index(index, index.numel(), "index");
   const c10::cuda::CUDAGuard guard(table.device());
   Tensor out = at::empty({index.numel(), table.size(1)}, table.options());
   done(sinkslot_lookup(ptr(table), dtype_code(table), table.stride(0), table.size(0),
@@ -86,8 +122,12 @@ Tensor lookup(const Tensor& table, const Tensor& index, double scale) {
 Tensor lookup_grad(const Tensor& grad_out, const Tensor& index, int64_t rows, double scale,
                    int64_t padding) {
   const c10::cuda::CUDAGuard guard(grad_out.device());
+  TORCH_CHECK_VALUE(grad_out.dim() == 2 && grad_out.size(0) == index.numel(),
+                    "grad_out: expected a row for each index");
+  expect_index(index, index.numel(), "index");
   const Tensor g = grad_out.stride(1) == 1 || grad_out.size(1) == 1 ? grad_out
                                                                      : grad_out.contiguous();
+  expect_rows(g, "grad_out");
   const int64_t dim = g.size(1), count = index.numel();
   int64_t bytes = 0;
   done(sinkslot_lookup_grad_workspace_bytes(count, rows, dim, &bytes), "lookup_grad");
@@ -103,6 +143,8 @@ Tensor lookup_grad(const Tensor& grad_out, const Tensor& index, int64_t rows, do
 std::tuple<Tensor, Tensor, Tensor> token_logprobs(const Tensor& z, const Tensor& tokens,
                                                   double temperature, int64_t ignore_index,
                                                   bool entropy) {
+  expect_rows(z, "logits");
+  expect_index(tokens, z.size(0), "tokens");
   const c10::cuda::CUDAGuard guard(z.device());
   const int64_t rows = z.size(0);
   Tensor logp = empty_f32({rows}, z), ent = empty_f32({entropy ? rows : 0}, z),
@@ -118,6 +160,15 @@ Tensor token_logprobs_grad(const Tensor& z, const Tensor& tokens, const Tensor& 
                            const Tensor& entropy, const optional<Tensor>& g,
                            const optional<Tensor>& g_entropy, double temperature,
                            int64_t ignore_index) {
+  expect_rows(z, "logits");
+  const int64_t rows = z.size(0);
+  expect_index(tokens, rows, "tokens");
+  expect(stats, at::kFloat, 2 * rows, "stats");
+  expect(entropy, at::kFloat, g_entropy.has_value() ? rows : entropy.numel(), "entropy");
+  for (const auto* t : {&g, &g_entropy})  // one value may stand for all rows
+    TORCH_CHECK_VALUE(!t->has_value() || ((*t)->is_cuda() && (*t)->scalar_type() == at::kFloat &&
+                                          (*t)->dim() == 1 && (*t)->numel() == rows),
+                      "outer gradient: expected one float32 for each row");
   const c10::cuda::CUDAGuard guard(z.device());
   Tensor out = grad_like(z);
   done(sinkslot_token_logprobs_grad(
@@ -130,21 +181,20 @@ Tensor token_logprobs_grad(const Tensor& z, const Tensor& tokens, const Tensor& 
   return out;
 }
 
-int64_t sequences(const optional<Tensor>& offsets) {
-  return offsets.has_value() ? offsets->numel() - 1 : 1;
-}
-int offset_bytes(const optional<Tensor>& offsets) {
-  return offsets.has_value() ? (int)offsets->element_size() : 8;
-}
-
 std::tuple<Tensor, Tensor> policy_loss(const Tensor& logp, const Tensor& old_logp,
                                        const Tensor& advantages, const optional<Tensor>& ref_logp,
                                        const optional<Tensor>& mask,
                                        const optional<Tensor>& offsets, bool adv_per_token,
                                        double clip_low, double clip_high, double kl_coef,
                                        int64_t kl, bool sequence_average, bool want_grad) {
-  const c10::cuda::CUDAGuard guard(logp.device());
+  expect_offsets(offsets);
   const int64_t t = logp.numel(), s = sequences(offsets);
+  expect(logp, at::kFloat, t, "logp");
+  expect(old_logp, at::kFloat, t, "old_logp");
+  expect(ref_logp, at::kFloat, t, "ref_logp");
+  expect(advantages, at::kFloat, adv_per_token ? t : s, "advantages");
+  expect(mask, at::kBool, t, "mask");
+  const c10::cuda::CUDAGuard guard(logp.device());
   int64_t bytes = 0;
   done(sinkslot_loss_workspace_bytes(s, &bytes), "policy_loss");
   Tensor ws = workspace(bytes, logp), values = empty_f32({4}, logp),
@@ -159,6 +209,9 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logp, const Tensor& old_log
 }
 
 Tensor scale_tokens(const Tensor& coef, const Tensor& values, const Tensor& g) {
+  expect(coef, at::kFloat, coef.numel(), "coef");
+  expect(values, at::kFloat, 4, "values");
+  expect(g, at::kFloat, 1, "outer gradient");
   const c10::cuda::CUDAGuard guard(coef.device());
   Tensor out = at::empty_like(coef);
   done(sinkslot_scale_tokens(f32(coef), coef.numel(), f32(values) + 3, f32(g), f32(out),
@@ -173,8 +226,15 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_logits(
     const optional<Tensor>& offsets, double temperature, bool adv_per_token, double clip_low,
     double clip_high, double kl_coef, int64_t kl, bool sequence_average, double grad_scale,
     bool want_grad) {
-  const c10::cuda::CUDAGuard guard(z.device());
+  expect_rows(z, "logits");
+  expect_offsets(offsets);
   const int64_t t = z.size(0), vocab = z.size(1), s = sequences(offsets);
+  expect_index(tokens, t, "tokens");
+  expect(old_logp, at::kFloat, t, "old_logp");
+  expect(ref_logp, at::kFloat, t, "ref_logp");
+  expect(advantages, at::kFloat, adv_per_token ? t : s, "advantages");
+  expect(mask, at::kBool, t, "mask");
+  const c10::cuda::CUDAGuard guard(z.device());
   int64_t bytes = 0;
   done(sinkslot_policy_logits_workspace_bytes(t, s, &bytes), "policy_loss_from_logits");
   Tensor ws = workspace(bytes, z), values = empty_f32({4}, z), logp = empty_f32({t}, z);
@@ -190,6 +250,8 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_logits(
 }
 
 void scale_rows_(Tensor grad, const Tensor& g, double grad_scale) {
+  expect_rows(grad, "grad");
+  expect(g, at::kFloat, 1, "outer gradient");
   const c10::cuda::CUDAGuard guard(grad.device());
   done(sinkslot_scale_rows(ptr(grad), dtype_code(grad), grad.stride(0), grad.size(0),
                            grad.size(1), f32(g), grad_scale, stream_of(grad)),
@@ -201,6 +263,10 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logp, const Ten
                                                    const optional<Tensor>& mask, double beta,
                                                    double smoothing, int64_t kind,
                                                    bool normalize) {
+  expect_offsets(offsets);
+  expect(logp, at::kFloat, logp.numel(), "logp");
+  expect(ref_logp, at::kFloat, logp.numel(), "ref_logp");
+  expect(mask, at::kBool, logp.numel(), "mask");
   const c10::cuda::CUDAGuard guard(logp.device());
   const int64_t s = offsets.numel() - 1;
   int64_t bytes = 0;
@@ -217,6 +283,10 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logp, const Ten
 
 Tensor preference_grad(const Tensor& slope, const Tensor& offsets, const optional<Tensor>& mask,
                        const Tensor& g, int64_t tokens) {
+  expect(slope, at::kFloat, slope.numel(), "slope");
+  expect_index(offsets, slope.numel() + 1, "offsets");
+  expect(mask, at::kBool, tokens, "mask");
+  expect(g, at::kFloat, 1, "outer gradient");
   const c10::cuda::CUDAGuard guard(slope.device());
   Tensor out = empty_f32({tokens}, slope);
   done(sinkslot_preference_grad(f32(slope), ptr<uint8_t>(mask), ptr(offsets),

@@ -785,6 +785,37 @@ def test_captured_large_paths(sk):
         assert torch.equal(a, b)
 
 
+def test_launching_operators_refuse_what_their_functions_never_pass(sk):
+    """Called directly: wrong types, sizes and layouts are errors before any launch."""
+    ops = torch.ops.sinkslot_b200
+    f, i = torch.randn(6, 8, device="cuda"), torch.zeros(6, dtype=torch.int64, device="cuda")
+    v, one = torch.zeros(6, device="cuda"), torch.ones((), device="cuda")
+    off = torch.tensor([0, 3, 6], device="cuda")
+    for call in [
+            lambda: ops.lookup(f.double(), i, 1.0),
+            lambda: ops.lookup(f.t(), i, 1.0),
+            lambda: ops.lookup(f, v, 1.0),
+            lambda: ops.lookup_grad(f, i[:5], 4, 1.0, -1),
+            lambda: ops.lookup_grad(f, i, 0, 1.0, -1),
+            lambda: ops.token_logprobs(f, i[:5], 1.0, -100, False),
+            lambda: ops.token_logprobs_grad(f, i, v, v, v, None, 1.0, -100),
+            lambda: ops.token_logprobs_grad(f, i, torch.zeros(6, 2, device="cuda"), v, v.half(), None,
+                                            1.0, -100),
+            lambda: ops.policy_loss(v, v[:5], v, None, None, off, True, 0.2, 0.2, 0.0, 3, False, True),
+            lambda: ops.policy_loss(v, v, v, None, None, off, False, 0.2, 0.2, 0.0, 3, False, True),
+            lambda: ops.policy_loss(v, v, v, None, v, off, True, 0.2, 0.2, 0.0, 3, False, True),
+            lambda: ops.policy_loss(v, v, v, None, None, off, True, 0.2, 0.2, 0.0, 4, False, True),
+            lambda: ops.scale_tokens(v, v, one),
+            lambda: ops.policy_loss_logits(f, i, v, v, None, None, off[:1], 1.0, True, 0.2, 0.2, 0.0,
+                                           3, False, 1.0, True),
+            lambda: ops.scale_rows_(f, v, 1.0),
+            lambda: ops.preference_loss(v.half(), off, None, None, 0.1, 0.0, 0, False),
+            lambda: ops.preference_loss(v, off[:2], None, None, 0.1, 0.0, 0, False),
+            lambda: ops.preference_grad(v, off, None, one, 6)]:
+        with pytest.raises(ValueError):
+            call()
+
+
 # ------------------------------------------------------------------ sizes past 32 bits
 def test_logits_of_more_than_2_to_the_31_elements(sk):
     """The last rows of 16400 x 131072 logits, through the log-probabilities' own kernels and the
