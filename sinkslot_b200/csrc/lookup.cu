@@ -74,10 +74,12 @@ __device__ __forceinline__ uint4 load16(const T* p, const T* begin, const T* end
 constexpr int kLookVecs = 4;
 
 // kAligned: all rows begin on 16-byte boundaries.  I: 32 bits where the output's
-// elements fit (a division of 64 bits costs more than the copy).
+// elements fit (a division of 64 bits costs more than the copy).  A thread's vectors
+// lie `skip` rows and `over` columns apart.
 template <typename T, typename I, bool kAligned>
 __global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restrict__ table,
                                                               int64_t stride, int64_t rows, I dim,
+                                                              I skip, I over,
                                                               const void* __restrict__ index,
                                                               int index_bytes, I total,
                                                               float scale, T* __restrict__ out) {
@@ -88,14 +90,21 @@ __global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restric
   int64_t r[kLookVecs], next[kLookVecs];
   I c[kLookVecs];
   uint4 u[kLookVecs], w[kLookVecs];
+  I t = v0 * N / dim, col = v0 * N - t * dim;
 #pragma unroll
   for (int k = 0; k < kLookVecs; ++k) {
     const I v = v0 + k * kLookThreads;
     r[k] = next[k] = -1;
-    c[k] = 0;
+    if (k > 0) {
+      t += skip;
+      col += over;
+      if (col >= dim) {
+        col -= dim;
+        ++t;
+      }
+    }
+    c[k] = col;
     if (v < vecs) {
-      const I t = v * N / dim;
-      c[k] = v * N - t * dim;
       r[k] = index_at(index, index_bytes, (int64_t)t);
       if (!kAligned && c[k] + N > dim) next[k] = index_at(index, index_bytes, (int64_t)t + 1);
     }
@@ -133,10 +142,10 @@ __global__ void __launch_bounds__(kLookThreads) lookup_kernel(const T* __restric
     reinterpret_cast<uint4*>(out)[v] = pack(f, (const T*)nullptr);
   }
   if (!kAligned && blockIdx.x == 0 && threadIdx.x < total - vecs * N) {
-    const I e = vecs * N + threadIdx.x, t = e / dim;
-    const int64_t row = index_at(index, index_bytes, (int64_t)t);
+    const I e = vecs * N + threadIdx.x, te = e / dim;
+    const int64_t row = index_at(index, index_bytes, (int64_t)te);
     out[e] = from_f32<T>(row >= 0 && row < rows
-                             ? to_f32(table[row * stride + (int64_t)(e - t * dim)]) * scale
+                             ? to_f32(table[row * stride + (int64_t)(e - te * dim)]) * scale
                              : __int_as_float(0x7fc00000));
   }
 }
@@ -176,7 +185,8 @@ static int launch_lookup(const void* table, int64_t stride, int64_t rows, int64_
   const bool narrow = total + kLookThreads * kLookVecs * N < (int64_t(1) << 32);
 #define GO(I, A)                                                                          \
   lookup_kernel<T, I, A><<<(unsigned)grid, kLookThreads, 0, st>>>(                        \
-      (const T*)table, stride, rows, (I)dim, index, index_bytes, (I)total, scale, (T*)out)
+      (const T*)table, stride, rows, (I)dim, (I)(kLookThreads * N / dim),                 \
+      (I)(kLookThreads * N % dim), index, index_bytes, (I)total, scale, (T*)out)
   if (rows16) {
     if (narrow) GO(uint32_t, true); else GO(int64_t, true);
   } else {
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(kLookThreads, 4) lookup_sum_kernel(SumArgs a,
 // (blockIdx.y): where there are fewer, its lanes share the row's windows as well.  Rows
 // over many windows are left to the CTA's warps together.  All sums are joined in an
 // order that the row's place alone decides.
-constexpr int kLongChain = 16;  // windows for each lane group of a warp
+constexpr int kLongChain = 4;  // windows for each lane group of a warp
 
 template <typename T, int VN>
 __global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a, int lanes,
@@ -722,8 +732,9 @@ __global__ void __launch_bounds__(kLookThreads) lookup_join_kernel(SumArgs a, in
   chain_enter();
   const uint32_t chains = a.chains[0];
   const int64_t windows = (a.count + a.window - 1) / a.window;
-  for (uint32_t item0 = blockIdx.x * kWarps; item0 < chains; item0 += gridDim.x * kWarps) {
-    const uint32_t item = item0 + warp;
+  // (CTA by CTA first, warp by warp then: a few rows go to as many CTAs)
+  for (uint32_t item0 = blockIdx.x; item0 < chains; item0 += gridDim.x * kWarps) {
+    const uint32_t item = item0 + gridDim.x * warp;
     int64_t w = 0, n = 0;
     uint32_t cur = 0;
     if (item < chains) {
@@ -838,7 +849,7 @@ static int launch_sums(SumArgs a, const void* g, void* out, cudaStream_t st) {
   int lanes = 1;
   while (lanes < 32 && lanes < a.ncv) lanes *= 2;
   int64_t x = ceil_div64(6 * num_sms(), groups);
-  if (x > ceil_div64(windows, kLookThreads / 32)) x = ceil_div64(windows, kLookThreads / 32);
+  if (x > windows) x = windows;
   SINKSLOT_CUDA_TRY(launch_chained(lookup_join_kernel<T, VN>, dim3((unsigned)x, (unsigned)groups),
                                    dim3(kLookThreads), 0, st, a, lanes, (T*)out));
   return kOk;

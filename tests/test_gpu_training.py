@@ -693,6 +693,26 @@ def test_streams_other_than_the_default(sk):
             assert torch.equal(a, b)
 
 
+def test_two_threads_at_once(sk):
+    """Each host thread on a stream of its own, at the same time: the results of one alone."""
+    from concurrent.futures import ThreadPoolExecutor
+    states = [_step_state(63), _step_state(64)]
+    want = [_step(sk, s) for s in states]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [_step(sk, states[k]) for _ in range(20)][-1]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with ThreadPoolExecutor(max_workers=2) as pool:
+        got = list(pool.map(work, range(2)))
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert torch.equal(a, b)
+
+
 def test_offsets_that_lie_stay_in_bounds(sk):
     """Offsets beyond the tokens, negative or falling: no access outside the tensors."""
     logp, old, refp, mask, _ = _tokens_of(70, 1000)
