@@ -2,18 +2,21 @@
 // rows gives each token's log-probability and its row's gradient, and the logits
 // are read from memory once.
 //
-// A cluster of CTAs takes a row, 32 KB of it for each CTA: it sums its slice, swaps
+// A cluster of CTAs takes a row, 64 KB of it for each CTA: it sums its slice, swaps
 // sums with the cluster through distributed shared memory, works out the token's
 // coefficient and turns its slice into the gradient, reading it again from L2, where
-// the slices under way (45 MB at 10 CTAs on each SM) stay: 314 MB came from memory
+// the slices under way (47 MB at 5 CTAs on each SM) stay: 314 MB came from memory
 // for 310 MB of logits.  Stores are marked to leave L2 first.
 //
-// Each CTA spends its time in turn on loads, on the swap and on stores, so many small
-// ones fill the memory's time best (8192 x 131072 bf16: 128 threads x 8, 9, 10 on an SM
-// 793, 796, 799 us, and 393, 381, 378 for 4096 x 65536 fp32; 256 x 4 983; whole rows by
-// 1024 threads 917).  Log-probabilities and gradient by their own kernels, three
-// passes, take 980.  What bounds it: exponentials (two for each element) hold their
-// unit for 66% of the time, and memory runs at 5.4 of 6.5 TB/s.
+// Each CTA spends its time in turn on loads, on the swap and on stores, so several fill
+// the memory's time best, as long as L2 holds them.  Threads x CTAs on an SM x KB, us
+// for 8192 x 131072 bf16, 8192 x 50021 fp16, 4096 x 65536 fp32:
+//   256 x 5 x 64  777 335 386     256 x 4 x 64  815 363 404     256 x 6 x 64  845 316 434
+//   128 x 10 x 32 802 372 379     128 x 8 x 64  925 344 479     512 x 2 x 128 826 371 412
+//   1024 x 1, whole rows          917 572 446
+//   log-probabilities and gradient by their own kernels, three passes: 988 391 495
+// What bounds it: exponentials (two for each element) hold their unit for 66% of the
+// time, and memory runs at 5.5 of 6.5 TB/s.
 //
 // A persistent form with the rows in shared memory (bulk copies in and out, warps by
 // role, sums exchanged a row ahead) was measured at 1013 us: a row's exchange took
@@ -30,9 +33,9 @@ namespace sinkslot {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSweepThreads = 128;
-constexpr int kSweepCtas = 10;                // on each SM
-constexpr int64_t kSweepBytes = 32 << 10;     // of a row, for each CTA
+constexpr int kSweepThreads = 256;
+constexpr int kSweepCtas = 5;              // on each SM
+constexpr int64_t kSweepBytes = 64 << 10;  // of a row, for each CTA
 constexpr int kMaxCluster = 8;
 
 template <typename T>
@@ -116,11 +119,13 @@ static int rows_split(const LogitRows& r) {
   return 0;
 }
 
+// From 24 KB a row on: 16384 rows of 32 KB 213 us (257 in three passes), of 16 KB 142
+// (129).
 bool policy_rows_fit(const LogitRows& r, const void* dz, int64_t dz_stride) {
   const int64_t size = dtype_bytes(r.dtype), row = r.vocab * size;
   const bool same = ((reinterpret_cast<uintptr_t>(r.z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0 &&
                     (r.stride - dz_stride) * size % 16 == 0;
-  return same && row >= 8192 && r.rows * row >= (128 << 20) && rows_split(r) > 0;
+  return same && row >= (24 << 10) && r.rows * row >= (128 << 20) && rows_split(r) > 0;
 }
 
 template <typename T>

@@ -457,8 +457,8 @@ def test_clip_is_decided_at_its_border(sk):
     (1, 17, 0, "token", 0), (40, 333, 3, "sequence", 5), (64, 50021, 3, "sequence", 0),
     (9, 32768, 2, "token", 64), (700, 4099, 12, "token", 1), (300, 130000, 4, "sequence", 0),
     (50, 262144, 1, "token", 0),
-    # logits larger than L2: rows that stay in shared memory, by 1, 2, 4 and 8 CTAs
-    (9100, 8233, 40, "sequence", 0), (2300, 32768, 5, "token", 64), (1400, 50021, 9, "sequence", 3),
+    # logits larger than L2: one pass over rows by 1, 2, 4 and 8 CTAs
+    (5600, 13001, 40, "sequence", 0), (2300, 32768, 5, "token", 64), (1400, 50021, 9, "sequence", 3),
     (1200, 131072, 16, "token", 0)])
 def test_policy_loss_from_logits(sk, t, vocab, count, average, pad, dtype):
     gen = _gen(t + vocab)
@@ -505,8 +505,12 @@ def test_policy_loss_from_logits(sk, t, vocab, count, average, pad, dtype):
     coef, = torch.autograd.grad(want, [leaf])
     coef = coef * scale
     wgrad = ref.logprobs_grad64(zd, tokens, coef, None, temperature) * mask[:, None]
+    # the coefficient is rA - 0.05 (e^gap - 1): where the two cancel (A = -0.0122 against a gap of 0.2
+    # leaves one part in 160), its error is that of the two, not one relative to what is left
+    made_of = ref.policy_coef_size(lp, old, adv, refp, mask, offsets, 0.05, average) * scale
+    onto = ref.logprobs_grad64(zd, tokens, made_of, None, temperature).abs() * mask[:, None]
     tol = _grad_tolerance(zd, tokens, coef, None, temperature, wgrad, dtype) \
-        + wgrad.abs() * (4 * float(ltol.max()) + 32 * EPS32)
+        + onto * (4 * float(ltol.max()) + 32 * EPS32)
     _close(grad, wgrad, tol, "grad")
     assert grad.stride() == z.stride() or t == 1
 

@@ -106,6 +106,25 @@ def policy64(logp, old, adv, ref=None, mask=None, offsets=None, lo=0.2, hi=0.2, 
     return loss, mean_kl, clipped / max(total, 1)
 
 
+def policy_coef_size(logp, old, adv, ref, mask, offsets, kl_coef, average):
+    """What a token's coefficient is made of: weight * (r |A| + kl_coef e^(ref - logp)).  An error
+    of logp goes into r and into e^gap relative to themselves, so the coefficient's own error is
+    that error (and the roundings) times this size, however much of it cancels."""
+    t = logp.numel()
+    o = [0, t] if offsets is None else [int(v) for v in offsets]
+    keep = torch.ones(t, dtype=torch.bool, device=logp.device) if mask is None else mask
+    size = torch.zeros(t, dtype=torch.float64, device=logp.device)
+    spans = [(a, b, int(keep[a:b].sum())) for a, b in zip(o[:-1], o[1:])]
+    total, used = sum(n for _, _, n in spans), sum(n > 0 for _, _, n in spans)
+    for i, (a, b, n) in enumerate(spans):
+        if n:
+            av = adv.double()[a:b] if adv.numel() == t else adv.double()[i]
+            part = torch.exp(logp[a:b] - old[a:b].double()) * av.abs() \
+                + kl_coef * torch.exp(ref[a:b].double() - logp[a:b])
+            size[a:b] = part * keep[a:b] / (total if average == "token" else n * used)
+    return size
+
+
 def preference64(logp, offsets, ref=None, mask=None, beta=0.1, smoothing=0.0, kind="sigmoid",
                  normalize=False):
     """(loss, rewards of all sequences) in 64 bits; differentiable in logp."""
