@@ -364,8 +364,8 @@ int sinkslot_dual_value(const float* phi, const float* a, int64_t n, const float
  * ------------------------------------------------------------------------- */
 
 /* out[t, :] = scale * table[index[t], :], out (count, dim) contiguous; index
- * int32 or int64 (index_bytes 4 or 8).  An index outside [0, rows) gives a row
- * of NaN. */
+ * int32 or int64 (index_bytes 4 or 8), out on a 16-byte boundary.  An index
+ * outside [0, rows) gives a row of NaN. */
 int sinkslot_lookup(const void* table, int dtype, int64_t stride, int64_t rows, int64_t dim,
                     const void* index, int index_bytes, int64_t count, double scale, void* out,
                     void* stream);
@@ -374,7 +374,8 @@ int sinkslot_lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t di
                                          int64_t* bytes_host);
 
 /* grad_table[v, :] = scale * sum of grad_out[t, :] over the t with index[t] = v,
- * (rows, dim) contiguous; rows that no index names are zeros.  Tokens whose
+ * (rows, dim) contiguous, on a 16-byte boundary; rows that no index names are
+ * zeros.  Tokens whose
  * index is `padding` (-1: none) or outside [0, rows) give nothing.  The order of
  * each sum follows from index alone. */
 int sinkslot_lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* index,

@@ -729,6 +729,32 @@ def test_offsets_that_lie_stay_in_bounds(sk):
     torch.cuda.synchronize()
 
 
+def test_without_recording(sk):
+    """no_grad, inference mode and inputs that need no gradient: the same values, nothing recorded."""
+    s = _step_state(65)
+
+    def values():
+        lp, h = sk.token_logprobs(s["z"], s["tokens"], entropy=True)
+        pol = sk.policy_loss(lp, s["old"], s["adv"], mask=s["mask"], offsets=s["offsets"])
+        pre = sk.preference_loss(lp, s["offsets"], mask=s["mask"])
+        fused = sk.policy_loss_from_logits(s["z"], s["tokens"], s["old"], s["adv"], mask=s["mask"],
+                                           offsets=s["offsets"])
+        return [sk.embedding_lookup(s["table"], s["ids"]), lp, h, *pol, *pre, *fused]
+
+    recorded = values()
+    assert [t.requires_grad for t in recorded] == [True, True, True, True, False, False, False, True,
+                                                   False, False, True, False, False, False]
+    with torch.no_grad():
+        plain = values()
+    with torch.inference_mode():
+        inferred = values()
+    s["z"], s["table"] = s["z"].detach(), s["table"].detach()
+    constant = values()
+    for a, *others in zip(recorded, plain, inferred, constant):
+        for b in others:
+            assert torch.equal(a, b) and not b.requires_grad
+
+
 def test_second_derivatives_are_refused(sk):
     """create_graph gives the first derivative; differentiating it again is an error."""
     gen = _gen(71)
