@@ -395,7 +395,8 @@ int sinkslot_token_logprobs(const void* logits, int dtype, int64_t stride, int64
 
 /* Gradient of the logits (same dtype, rows grad_stride apart) for the outer
  * gradients g of logp and g_entropy of entropy (each nullable, not both; strides
- * 0 or more).  entropy: the forward's output, needed with g_entropy. */
+ * 0 or more).  Rows whose outer gradients are 0 get zeros, whatever they hold.
+ * entropy: the forward's output, needed with g_entropy. */
 int sinkslot_token_logprobs_grad(const void* logits, int dtype, int64_t stride, int64_t rows,
                                  int64_t vocab, const void* tokens, int token_bytes,
                                  int64_t ignore, double inv_temp, const float* stats,

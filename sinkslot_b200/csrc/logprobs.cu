@@ -200,23 +200,24 @@ __global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogitRows r, 
   const int body = (int)row_span(out, r.vocab).body;
   const int v0 = min(body, share * (int)blockIdx.y), v1 = min(body, v0 + share);
   const bool edges = blockIdx.y == 0;
-  if (tok == r.ignore || (r.mask && !r.mask[row])) {
-    write_zeros(out, r.vocab, v0, v1, edges, threadIdx.x, kRowThreads);
-    return;
-  }
   RowCoef q;
   const float2 ms = g.stats[row];
   q.inv_temp = (float)r.inv_temp;
   float f = q.inv_temp * g.scale;
   if (g.scale_dev) f *= g.scale_dev[0];
   const float gp = g.g ? g.g[row * g.g_stride] * f : 0.0f;
+  const float ge = kEnt && g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] * f : 0.0f;
+  // no gradient: zeros, whatever the row holds (0 * NaN is not taken)
+  if (tok == r.ignore || (r.mask && !r.mask[row]) || (gp == 0.0f && ge == 0.0f)) {
+    write_zeros(out, r.vocab, v0, v1, edges, threadIdx.x, kRowThreads);
+    return;
+  }
   const float rs = inverse_sum(ms.y);
   q.m = ms.x;
   q.c = (float)(r.inv_temp * 1.4426950408889634);
   q.cp = -gp * rs;
   q.ce = q.k = 0.0f;
   if (kEnt) {
-    const float ge = g.g_entropy ? g.g_entropy[row * g.g_entropy_stride] * f : 0.0f;
     q.ce = -ge * rs;
     q.k = ms.y > 0.0f ? g.entropy[row] - logf(ms.y) : 0.0f;
   }

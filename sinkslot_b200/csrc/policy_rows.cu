@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(kSweepThreads, kSweepCtas) policy_rows_kernel(
   __shared__ Online warp_part[kWarps];
   __shared__ Online cta_part[kMaxCluster];
   __shared__ RowCoef coef;
+  __shared__ bool idle;
   const int64_t row = blockIdx.x / (unsigned)split;
   const int rank = (int)(blockIdx.x % (unsigned)split);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -104,8 +105,13 @@ __global__ void __launch_bounds__(kSweepThreads, kSweepCtas) policy_rows_kernel(
     q.cp = -g * inverse_sum(o.s);
     q.hit = o.s == 0.0f ? 0.0f : g;
     coef = q;
+    idle = g == 0.0f;
   }
   __syncthreads();
+  if (idle) {  // no gradient (outside the sequences, or clipped): zeros, whatever the row holds
+    write_zeros(out, r.vocab, v0, v1, rank == 0, threadIdx.x, kSweepThreads);
+    return;
+  }
   const RowCoef q = coef;
   write_grad<T, false>(p, out, r.vocab, v0, v1, rank == 0, true, threadIdx.x, kSweepThreads, tok,
                        q);

@@ -23,7 +23,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: floa
     ``ignore_index`` give 0, get a gradient of 0 and are not read.  Any other
     token outside the vocabulary gives NaN.  Logits of -inf are impossible
     tokens: probability 0, gradient 0; a row of nothing else gives -inf, entropy
-    0 and gradient 0.
+    0 and gradient 0.  A row whose outer gradients are 0 gets zeros, whatever it
+    holds.
     """
     logp, ent = torch_ops().logprobs(logits, tokens, temperature, ignore_index, entropy)
     return (logp, ent) if entropy else logp

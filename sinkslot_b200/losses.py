@@ -72,7 +72,8 @@ def policy_loss_from_logits(logits: torch.Tensor, tokens: torch.Tensor, old_logp
 
     ``logits``: (tokens, vocab), float32, float16 or bfloat16; the other
     arguments as in :func:`token_logprobs` and :func:`policy_loss`.  Rows with
-    ``mask`` False are not read; their log-probability is given as 0.
+    ``mask`` False are not read; their log-probability is given as 0.  Rows of
+    tokens that get no gradient get zeros, whatever they hold.
 
     The gradient is held in the logits' type until the backward pass, which runs
     once.  It is made for a loss multiplied by ``grad_scale``: where the outer

@@ -755,6 +755,35 @@ def test_without_recording(sk):
             assert torch.equal(a, b) and not b.requires_grad
 
 
+@pytest.mark.parametrize("t,vocab", [(40, 1003), (5600, 13001)])  # three passes; one pass
+def test_rows_without_gradient_may_hold_anything(sk, t, vocab):
+    """Tokens outside the sequences, and tokens whose gradient is zero: NaN and infinities in their
+    rows reach nothing, and the gradients of their rows are zeros."""
+    gen = _gen(t)
+    z = torch.randn(t, vocab, generator=gen, device="cuda").half()
+    tokens = torch.randint(0, vocab, (t,), generator=gen, device="cuda")
+    old = torch.full((t,), -7.0, device="cuda")
+    adv = torch.ones(2, device="cuda")
+    offsets = torch.tensor([3, 20, t - 5], device="cuda")
+    inside = torch.zeros(t, dtype=torch.bool, device="cuda")
+    inside[3:t - 5] = True
+    z[0], z[1], z[t - 1] = math.nan, math.inf, -math.inf
+    z[t - 2, 7] = math.nan
+    z.requires_grad_()
+    fused = sk.policy_loss_from_logits(z, tokens, old, adv, clip_high=9.0, offsets=offsets)
+    grad, = torch.autograd.grad(fused.loss, [z])
+    lp = sk.token_logprobs(z, tokens)
+    loss = sk.policy_loss(lp, old, adv, clip_high=9.0, offsets=offsets).loss
+    split, = torch.autograd.grad(loss, [z])
+    assert fused.loss.isfinite()
+    for g in (grad, split):
+        assert not g[~inside].any() and g[inside].isfinite().all() and g[inside].any()
+    lp, h = sk.token_logprobs(z, tokens, entropy=True)
+    for part in (lp[inside].sum(), h[inside].sum(), (lp[inside] + h[inside]).sum()):
+        g, = torch.autograd.grad(part, [z], retain_graph=True)
+        assert not g[~inside].any() and g[inside].isfinite().all() and g[inside].any()
+
+
 def test_second_derivatives_are_refused(sk):
     """create_graph gives the first derivative; differentiating it again is an error."""
     gen = _gen(71)
