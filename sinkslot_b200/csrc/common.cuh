@@ -113,6 +113,16 @@ __device__ __forceinline__ T ld_stream(const T* p) {
   return __ldcs(p);
 }
 
+// A CTA's shared memory may be reached by its cluster once the CTA has started: all
+// threads of the cluster pass the first of these early on, and the second before the
+// first access to another CTA's memory (in turn with the cluster's other barriers).
+__device__ __forceinline__ void cluster_started() {
+  asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started() {
+  asm volatile("barrier.cluster.wait;\n" ::: "memory");
+}
+
 // Programmatic dependent launch.  The solve loop's half-step kernels are
 // launched so that each may be scheduled before the one ahead of it has
 // finished (launch_chained below).  Every such kernel waits, before it reads or

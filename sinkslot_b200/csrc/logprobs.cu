@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_row_kernel(LogitRows r, i
     }
     return;
   }
+  if (split > 1) cluster_started();
   const T* p = static_cast<const T*>(r.z) + row * r.stride;
   const Scale2 c = r.scale;
   Online o;
@@ -95,6 +96,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_row_kernel(LogitRows r, i
   join_warp<kEnt>(o, c);
   if (lane == 0) warp_part[warp] = o;
   __syncthreads();
+  if (split > 1) cluster_wait_started();
   if (warp == 0) {
     o = warp_part[lane & (kRowThreads / 32 - 1)];
     if (lane >= kRowThreads / 32) o = Online();

@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
     if (at < zero_tail) reinterpret_cast<uint16_t*>(zeros + zero_vecs)[at] = 0;
     return;
   }
+  cluster_started();
   extern __shared__ __align__(16) unsigned char raw[];
   SortShared& sh = *reinterpret_cast<SortShared*>(raw);
   uint2* buf = reinterpret_cast<uint2*>(raw + sizeof(SortShared));  // (row, token) twice
@@ -303,6 +304,7 @@ __global__ void __launch_bounds__(kSortCta, 1) lookup_sort_kernel(
       loc[r] = (uint16_t)(base + before);
     }
     __syncthreads();
+    if (shift == 0) cluster_wait_started();
     if (threadIdx.x < kDigits) {
       uint32_t sum = 0;
 #pragma unroll 8

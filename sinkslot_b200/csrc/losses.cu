@@ -51,13 +51,15 @@ __device__ __forceinline__ Sums warp_sums(Sums v) {
   return v;
 }
 
+// (`first`: the kernel's first call; it began with cluster_started() where split > 1)
 __device__ __forceinline__ Sums cluster_sums(Sums v, ClusterSum& sh, int turn, int rank,
-                                             int split) {
+                                             int split, bool first = false) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_sums(v);
   __syncthreads();
   if (lane == 0) sh.warp[warp] = v;
   __syncthreads();
+  if (first && split > 1) cluster_wait_started();
   if (warp == 0) {
     const Sums zero = {0.0, 0.0, 0.0};
     v = warp_sums(lane < kLossWarps ? sh.warp[lane] : zero);
@@ -120,7 +122,7 @@ __device__ __forceinline__ void policy_seq(const Packed& p, const PolicyTerms& t
       int64_t k = 0;
 #pragma unroll 4
       for (int64_t i = lo + at; i < hi; i += step) k += p.mask[i] != 0;
-      n = cluster_sums({(double)k, 0.0, 0.0}, sh, 0, rank, split).a;
+      n = cluster_sums({(double)k, 0.0, 0.0}, sh, 0, rank, split, true).a;
     }
     inv = n > 0.0 ? 1.0 / n : 0.0;
   }
@@ -165,7 +167,7 @@ __device__ __forceinline__ void policy_seq(const Packed& p, const PolicyTerms& t
   zero_outside(p, seq, at, step, coef);
   // counts of counted and of clipped tokens, both under 2^32, apart in fp64
   s.c = (double)(n & 0xffffffff);
-  const Sums f = cluster_sums(s, sh, 1, rank, split);
+  const Sums f = cluster_sums(s, sh, 1, rank, split, !(t.sequence_average && p.mask));
   const Sums k = cluster_sums({(double)(n >> 32), 0.0, 0.0}, sh, 0, rank, split);
   if (rank == 0 && threadIdx.x == 0) part[seq] = make_double4(f.a * inv, f.b * inv, k.a, f.c);
 }
@@ -175,6 +177,7 @@ __global__ void __launch_bounds__(kLossThreads) policy_seq_kernel(Packed p, Poli
                                                                   double4* __restrict__ part,
                                                                   float* __restrict__ coef) {
   __shared__ ClusterSum sh;
+  if (split > 1) cluster_started();
   policy_seq(p, t, e, blockIdx.x / (unsigned)split, (int)(blockIdx.x % (unsigned)split), split, sh,
              part, coef);
   chain_release();
@@ -337,7 +340,7 @@ __device__ __forceinline__ void preference_seq(const Packed& p, const float* __r
       }
   }
   s.b = (double)n;
-  const Sums f = cluster_sums(s, sh, 0, rank, split);
+  const Sums f = cluster_sums(s, sh, 0, rank, split, true);
   if (rank == 0 && threadIdx.x == 0) part[seq] = make_double2(f.a, f.b);
 }
 
@@ -345,6 +348,7 @@ __global__ void __launch_bounds__(kLossThreads) preference_seq_kernel(
     Packed p, const float* __restrict__ logp, const float* __restrict__ ref, int split,
     double2* __restrict__ part) {
   __shared__ ClusterSum sh;
+  if (split > 1) cluster_started();
   preference_seq(p, logp, ref, blockIdx.x / (unsigned)split, (int)(blockIdx.x % (unsigned)split),
                  split, sh, part);
   chain_release();
@@ -506,6 +510,7 @@ __global__ void __launch_bounds__(kLossThreads) policy_count_kernel(Packed p, in
                                                                     int64_t* __restrict__ counts,
                                                                     int* __restrict__ owner) {
   __shared__ ClusterSum sh;
+  if (split > 1) cluster_started();
   const int64_t seq = blockIdx.x / (unsigned)split;
   const int rank = (int)(blockIdx.x % (unsigned)split);
   const int64_t at = (int64_t)rank * kLossThreads + threadIdx.x;
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(kLossThreads) policy_count_kernel(Packed p, in
     for (int64_t i = at, e = offset_at(p, 0); i < e; i += step) owner[i] = -1;
   if (p.offsets && seq == p.count - 1)
     for (int64_t i = offset_at(p, p.count) + at; i < p.tokens; i += step) owner[i] = -1;
-  const Sums f = cluster_sums({(double)n, 0.0, 0.0}, sh, 0, rank, split);
+  const Sums f = cluster_sums({(double)n, 0.0, 0.0}, sh, 0, rank, split, true);
   if (rank == 0 && threadIdx.x == 0) counts[seq] = (int64_t)f.a;
   chain_release();
 }

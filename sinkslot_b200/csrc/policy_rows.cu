@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kSweepThreads, kSweepCtas) policy_rows_kernel(
     write_zeros(out, r.vocab, v0, v1, rank == 0, threadIdx.x, kSweepThreads);
     return;
   }
+  if (split > 1) cluster_started();
   const int64_t tok = token_at(r.tokens, r.token_bytes, row);
   const bool inside = tok >= 0 && tok < r.vocab;
   // what the coefficient needs besides the sums, on its way while the row is read
@@ -80,6 +81,7 @@ __global__ void __launch_bounds__(kSweepThreads, kSweepCtas) policy_rows_kernel(
   join_warp<false>(o, r.scale);
   if (lane == 0) warp_part[warp] = o;
   __syncthreads();
+  if (split > 1) cluster_wait_started();
   if (warp == 0) {
     o = lane < kWarps ? warp_part[lane] : Online();
     join_warp<false>(o, r.scale);
