@@ -8,7 +8,8 @@
 // their order), cut into windows of equal length whatever the rows' counts, and
 // each thread adds up one column vector of one window.  Rows that lie in one
 // window are written at once; rows that cross windows leave partial sums, which a
-// second kernel joins.  Rows that no token names are zeros.
+// second kernel joins.  Rows that no token names are zeros.  Few rows or few tokens
+// need no sort: each row looks for its own.
 //
 // Memory traffic bounds it: every token's gradient row is read once, the table's
 // gradient is written once (and the rows that are used once more).  Up to 90112
@@ -936,6 +937,121 @@ static int sort_tokens(const void* index, int index_bytes, int64_t count, int64_
   return kOk;
 }
 
+// --------------------------------------------------------------------------
+// Few rows or few tokens: one launch.  A CTA for each row of the table (and 256 of its
+// columns) looks through all indices, lists the tokens that name the row, and adds
+// their gradients up: `lanes` threads for the columns, the others take every
+// (256 / lanes)th token of the list; their sums are joined as a tree.  The order
+// follows from the indices alone.
+// --------------------------------------------------------------------------
+constexpr int kRowScan = 8;  // indices under way for each thread
+constexpr int kRowTile = kRowScan * kLookThreads;
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(kLookThreads) lookup_row_sum_kernel(
+    const I* __restrict__ index, int count, int64_t padding, const T* __restrict__ g,
+    int64_t stride, int64_t dim, int lanes, float scale, T* __restrict__ out) {
+  constexpr int kWarps = kLookThreads / 32;
+  __shared__ int list[2][kRowTile];
+  __shared__ int found[2][kWarps];
+  __shared__ float part[kLookThreads];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slice = threadIdx.x / (unsigned)lanes, slices = kLookThreads / lanes;
+  const int64_t col = (int64_t)blockIdx.y * kLookThreads + (threadIdx.x & (lanes - 1));
+  const bool on = col < dim;
+  const T* at = g + (on ? col : 0);
+  float sum = 0.0f;
+  const int end = row == padding ? 0 : count;
+  for (int first = 0, turn = 0; first < end; first += kRowTile, turn ^= 1) {
+    I idx[kRowScan];
+#pragma unroll
+    for (int k = 0; k < kRowScan; ++k) {
+      const int i = first + k * kLookThreads + (int)threadIdx.x;
+      idx[k] = i < end ? __ldg(index + i) : (I)-1;
+    }
+    uint32_t hits[kRowScan];
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kRowScan; ++k) {
+      hits[k] = __ballot_sync(0xffffffffu, (int64_t)idx[k] == row);
+      mine += __popc(hits[k]);
+    }
+    if (lane == 0) found[turn][warp] = mine;
+    __syncthreads();
+    int to = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) to = n;
+      n += found[turn][w];
+    }
+    if (n == 0) continue;
+#pragma unroll
+    for (int k = 0; k < kRowScan; ++k) {
+      if (hits[k] >> lane & 1)
+        list[turn][to + __popc(hits[k] & ((1u << lane) - 1u))] =
+            first + k * kLookThreads + (int)threadIdx.x;
+      to += __popc(hits[k]);
+    }
+    __syncthreads();  // (the next tile writes the other list)
+    int j = slice;
+    for (; j + 7 * slices < n; j += 8 * slices) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = to_f32(at[list[turn][j + k * slices] * stride]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[k];
+    }
+    for (; j < n; j += slices) sum += to_f32(at[list[turn][j] * stride]);
+  }
+  if (slices > 1) {
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    for (int k = slices / 2; k >= 1; k /= 2) {
+      if (slice < k) part[threadIdx.x] += part[threadIdx.x + k * lanes];
+      __syncthreads();
+    }
+    sum = part[threadIdx.x];
+  }
+  if (on && slice == 0) out[row * dim + col] = from_f32<T>(sum * scale);
+}
+
+static int lanes_of(int64_t dim) {
+  int lanes = 1;
+  while (lanes < kLookThreads && lanes < dim) lanes *= 2;
+  return lanes;
+}
+
+// Against the sort, us for the gradient (tokens spread evenly, and all on one row):
+//   256 x 3, 10000 tokens      6.1 (16.6), 11.1 (14.6)     512 x 512, 512   4.5 (14.8), 19.6 (14.6)
+//   50 x 771, 256              3.3 (14.4), 10.9 (13.8)     64 x 8, 16384    9.0 (19.2), 24.1 (15.2)
+//   4096 x 256, 256            8.9 (12.1), 12.5 (13.9)     8192 x 256, 256  15.7 (12.7)
+//   2048 x 4, 8192            17.8 (22.0), 12.8 (17.5)     16384 x 64, 64   31.9 (11.3)
+// The first limit bounds what one row's tokens may cost, the second the CTAs' launch
+// and the third the indices that are read.
+static bool few_rows(int64_t count, int64_t rows, int64_t dim) {
+  const int64_t ctas = rows * ceil_div64(dim, kLookThreads);
+  return count * lanes_of(dim) <= (int64_t(1) << 16) && ctas <= 4096 &&
+         ctas * count <= (int64_t(1) << 23);
+}
+
+template <typename T>
+static int launch_row_sums(const void* index, int index_bytes, int64_t count, int64_t rows,
+                           int64_t dim, int64_t padding, const void* g, int64_t stride,
+                           float scale, void* out, cudaStream_t st) {
+  const dim3 grid((unsigned)rows, (unsigned)ceil_div64(dim, kLookThreads));
+  if (index_bytes == 8)
+    lookup_row_sum_kernel<T, int64_t><<<grid, kLookThreads, 0, st>>>(
+        (const int64_t*)index, (int)count, padding, (const T*)g, stride, dim, lanes_of(dim), scale,
+        (T*)out);
+  else
+    lookup_row_sum_kernel<T, int32_t><<<grid, kLookThreads, 0, st>>>(
+        (const int32_t*)index, (int)count, padding, (const T*)g, stride, dim, lanes_of(dim), scale,
+        (T*)out);
+  SINKSLOT_CHECK_LAUNCH();
+  return kOk;
+}
+
 int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* index,
                 int index_bytes, int64_t count, int64_t rows, int64_t dim, double scale,
                 int64_t padding, void* grad_table, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -960,6 +1076,15 @@ int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* ind
   if (!cv.ok) {
     set_error("lookup_grad: workspace too small");
     return kWorkspaceTooSmall;
+  }
+  if (few_rows(count, rows, dim)) {
+#define GO(T)                                                                                \
+  return launch_row_sums<T>(index, index_bytes, count, rows, dim, padding, grad_out, stride, \
+                            (float)scale, grad_table, st)
+    if (dtype == kF32) GO(float);
+    if (dtype == kF16) GO(__half);
+    GO(__nv_bfloat16);
+#undef GO
   }
   SumArgs a = {};
   SINKSLOT_TRY(sort_tokens(index, index_bytes, count, rows, padding, grad_table, out_bytes, w,

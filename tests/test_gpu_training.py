@@ -260,6 +260,19 @@ def test_lookup_sizes(sk, rows, dim, tokens, dtype):
     _check_lookup(sk, table, index, 1.0 if tokens % 2 else 13.7)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,tokens", [  # on both sides of where the sort begins
+    (100, 3, 16384), (100, 3, 16385), (9, 256, 256), (9, 256, 257), (9, 300, 256), (4096, 5, 300),
+    (4097, 5, 300), (1024, 4, 8192), (1024, 4, 8193), (2, 1, 65536), (1, 129, 255), (2048, 512, 7)])
+def test_lookup_few_rows(sk, rows, dim, tokens, dtype):
+    gen = _gen(rows * dim + tokens)
+    table = torch.randn(rows, dim, generator=gen, device="cuda").to(dtype)
+    index = torch.randint(-2, rows + 2, (tokens,), generator=gen, device="cuda")
+    _check_lookup(sk, table.clone(), index, 3.3, padding=rows // 2)
+    _check_lookup(sk, table.clone(), index.int(), 1.0)
+    _check_lookup(sk, table.clone(), torch.full_like(index, rows - 1), 0.7)
+
+
 def test_lookup_one_hot_row_and_runs_at_window_ends(sk):
     gen = _gen(5)
     table = torch.randn(40, 20, generator=gen, device="cuda")
