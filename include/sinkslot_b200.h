@@ -375,9 +375,8 @@ int sinkslot_lookup_grad_workspace_bytes(int64_t count, int64_t rows, int64_t di
 
 /* grad_table[v, :] = scale * sum of grad_out[t, :] over the t with index[t] = v,
  * (rows, dim) contiguous, on a 16-byte boundary; rows that no index names are
- * zeros.  Tokens whose
- * index is `padding` (-1: none) or outside [0, rows) give nothing.  The order of
- * each sum follows from index alone. */
+ * zeros.  Tokens whose index is `padding` (-1: none) or outside [0, rows) give
+ * nothing.  The order of each sum follows from index alone. */
 int sinkslot_lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* index,
                          int index_bytes, int64_t count, int64_t rows, int64_t dim, double scale,
                          int64_t padding, void* grad_table, void* workspace,
