@@ -10,6 +10,7 @@
 // outputs), and the functions users call, which check, record the gradient and
 // call the former (any dispatch mode, fake tensors among them).
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -478,6 +479,14 @@ struct PreferenceLossFn : Function<PreferenceLossFn> {
 
 bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// A tangent would be lost where nothing is recorded: none of the functions has a
+// forward-mode derivative, and says so.
+void refuse_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(/*level=*/0).defined(),
+      name, ": forward-mode derivatives are not implemented");
+}
+
 // ---------------------------------------------------------------------------
 // Checks
 // ---------------------------------------------------------------------------
@@ -500,6 +509,7 @@ void check_index(const char* name, const char* what, const Tensor& t) {
                     " must be int32 or int64, got ", d);
 }
 void check_constant(const char* name, const char* what, const Tensor& t) {
+  refuse_tangent(name, t);
   TORCH_CHECK_VALUE(!records(t), name, ": no gradient is taken in ", what, "; detach it");
 }
 // One float32 value for each token, contiguous.
@@ -533,6 +543,7 @@ void check_logits(const char* name, const Tensor& logits, const Tensor& tokens,
                     ": tokens must have the shape ", logits.sizes().slice(0, logits.dim() - 1),
                     " of the logits' rows, got ", tokens.sizes());
   check_device(name, logits, logits);
+  refuse_tangent(name, logits);
   check_device(name, tokens, logits);
   check_dtype(name, "logits", logits);
   check_index(name, "tokens", tokens);
@@ -558,6 +569,7 @@ PolicyInputs check_policy(const char* name, const Tensor& like, const Tensor& ol
                           double clip_low, double clip_high, double kl_coef, c10::string_view kl,
                           c10::string_view average) {
   check_device(name, like, like);
+  refuse_tangent(name, like);  // (the log-probabilities, or whole-numbered tokens)
   check_device(name, old_logp, like);
   check_device(name, advantages, like);
   check_device(name, ref_logp, like);
@@ -600,6 +612,7 @@ Tensor embedding_lookup(const Tensor& table_, const Tensor& index, double scale,
   TORCH_CHECK_VALUE(table_.dim() == 2 && table_.size(0) >= 1 && table_.size(1) >= 1, name,
                     ": table must be (rows, dim), got ", table_.sizes());
   check_device(name, table_, table_);
+  refuse_tangent(name, table_);
   check_device(name, index, table_);
   check_dtype(name, "table", table_);
   check_index(name, "index", index);
@@ -709,6 +722,7 @@ std::tuple<Tensor, Tensor> preference(const Tensor& logp, const Tensor& offsets_
   const char* name = "preference_loss";
   TORCH_CHECK_VALUE(logp.dim() == 1, name, ": logp must be (tokens,), got ", logp.sizes());
   check_device(name, logp, logp);
+  refuse_tangent(name, logp);
   check_device(name, offsets_, logp);
   check_device(name, ref_logp_, logp);
   check_device(name, mask_, logp);

@@ -1,0 +1,60 @@
+"""The training operators under PyTorch's modes of differentiation, without a GPU (on fake CUDA
+tensors, which no kernel sees)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import sinkslot_b200 as sk
+
+
+@pytest.fixture
+def fake():
+    with FakeTensorMode():
+        yield
+
+
+def _cuda(*shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+def _calls():
+    """(name, the function of one floating argument, that argument's shape), for every floating
+    argument of every function."""
+    ids, off = _cuda(8, dtype=torch.int64), _cuda(3, dtype=torch.int64)
+    v, z = _cuda(8), _cuda(8, 30)
+    return [
+        ("table", lambda t: sk.embedding_lookup(t, ids), (20, 4)),
+        ("logits", lambda t: sk.token_logprobs(t, ids), (8, 30)),
+        ("logits, entropy", lambda t: sk.token_logprobs(t, ids, entropy=True)[1], (8, 30)),
+        ("logp", lambda t: sk.policy_loss(t, v, v).loss, (8,)),
+        ("old_logp", lambda t: sk.policy_loss(v, t, v).loss, (8,)),
+        ("advantages", lambda t: sk.policy_loss(v, v, t).loss, (8,)),
+        ("ref_logp", lambda t: sk.policy_loss(v, v, v, ref_logp=t, kl_coef=0.1).loss, (8,)),
+        ("policy logits", lambda t: sk.policy_loss_from_logits(t, ids, v, v).loss, (8, 30)),
+        ("policy old_logp", lambda t: sk.policy_loss_from_logits(z, ids, t, v).loss, (8,)),
+        ("policy advantages", lambda t: sk.policy_loss_from_logits(z, ids, v, t).loss, (8,)),
+        ("preference logp", lambda t: sk.preference_loss(t, off).loss, (8,)),
+        ("preference ref_logp", lambda t: sk.preference_loss(v, off, ref_logp=t).loss, (8,)),
+    ]
+
+
+def test_forward_mode_is_refused(fake):
+    """A tangent is never dropped, whether or not the call records a gradient."""
+    for name, call, shape in _calls():
+        with fwd.dual_level():
+            dual = fwd.make_dual(_cuda(*shape), _cuda(*shape))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+            leaf = _cuda(*shape).requires_grad_()
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fwd.make_dual(leaf, _cuda(*shape)))
+            call(fwd.unpack_dual(dual).primal)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (_cuda(*shape),), (_cuda(*shape),))
+        call(_cuda(*shape))
