@@ -218,9 +218,10 @@ __global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogitRows r, 
   q.m = ms.x;
   q.c = (float)(r.inv_temp * 1.4426950408889634);
   q.cp = -gp * rs;
-  q.ce = q.k = 0.0f;
+  q.ce = q.k = q.low = 0.0f;
   if (kEnt) {
     q.ce = -ge * rs;
+    q.low = exp_low(q.inv_temp);
     q.k = ms.y > 0.0f ? g.entropy[row] - logf(ms.y) : 0.0f;
   }
   q.hit = ms.y == 0.0f ? 0.0f : gp;

@@ -21,6 +21,14 @@ __device__ __forceinline__ float exp_scaled(float d, Scale2 c) {
   return exp2_fast(fmaf(d, c.hi, d * c.lo));
 }
 
+// The difference z - m, in logit units, from which on exp((z - m) / T) is 0 for sure
+// (exp2_fast flushes under 2^-126, from -87.4 T on).  Where the exponential
+// is multiplied by its own argument, the difference is held at it: 0 times an infinite
+// difference, or one that 1 / T or an outer gradient makes infinite, is NaN.  (A bound
+// without T in it, -1e30, was infinite once it had been scaled: T under 3e-9, or 0.01
+// under a loss scale of 2^17.)
+__host__ __device__ inline float exp_low(float inv_temp) { return -128.0f / inv_temp; }
+
 // Running (max, sum of exp(z - max), sum of exp(z - max) (z - max)); differences
 // in logit units, exponents in base 2.
 struct Online {
@@ -58,7 +66,7 @@ __device__ __forceinline__ void absorb(Online& o, const uint4 (&u)[U], Scale2 c)
       s = add2(s, e);
       if (kEnt) {  // exp(-inf) * -inf counts as 0
         const float2 t = parts(d);
-        w = fma2(e, pair(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), w);
+        w = fma2(e, pair(fmaxf(t.x, c.low), fmaxf(t.y, c.low)), w);
       }
     }
   }
@@ -165,7 +173,7 @@ __device__ __forceinline__ void read_row(Online& o, const T* __restrict__ p, int
     if (tid < edge) {
       const float d = f - o.m, x = exp_scaled(d, c);
       o.s += x;
-      if (kEnt) o.w = fmaf(x, fmaxf(d, -1e30f), o.w);
+      if (kEnt) o.w = fmaf(x, fmaxf(d, c.low), o.w);
     }
   }
 }
@@ -174,6 +182,7 @@ struct RowCoef {
   float m, c;       // exponent: (z - m) * c
   float cp, ce, k;  // d = e * (cp + ce * ((z - m) * inv_temp + k))
   float inv_temp;
+  float low;  // what z - m counts as where it is less (exp_low)
   float hit;  // added at the token
 };
 
@@ -182,7 +191,7 @@ __device__ __forceinline__ float grad_at(float z, const RowCoef& q) {
   const float d = z - q.m;
   const float e = exp2_fast(d * q.c);
   if (!kEnt) return e * q.cp;
-  return e * fmaf(q.ce, fmaf(fmaxf(d, -1e30f), q.inv_temp, q.k), q.cp);
+  return e * fmaf(q.ce, fmaf(fmaxf(d, q.low), q.inv_temp, q.k), q.cp);
 }
 
 template <typename T, bool kEnt>
@@ -201,7 +210,7 @@ __device__ __forceinline__ uint4 grad_vec(const uint4& u, const RowCoef& q) {
       r = parts(mul2(e, cp));
     } else {
       const float2 t = parts(d);
-      const f32x2 l = fma2(pair(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)),
+      const f32x2 l = fma2(pair(fmaxf(t.x, q.low), fmaxf(t.y, q.low)),
                            pair(q.inv_temp, q.inv_temp), pair(q.k, q.k));
       r = parts(mul2(e, fma2(pair(q.ce, q.ce), l, cp)));
     }
@@ -289,6 +298,7 @@ inline Scale2 scale2(double inv_temp) {
   Scale2 c;
   halves(inv_temp * 1.4426950408889634, c.hi, c.lo);
   halves(inv_temp, c.inv, c.inv_lo);
+  c.low = exp_low(c.inv);
   return c;
 }
 

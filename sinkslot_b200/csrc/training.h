@@ -24,9 +24,10 @@ int lookup_grad(const void* grad_out, int dtype, int64_t stride, const void* ind
                 int64_t padding, void* grad_table, void* ws, size_t ws_bytes, cudaStream_t st);
 
 // ---- logprobs.cu -----------------------------------------------------------
-// log2(e) / T and 1 / T, each as the sum of two floats.
+// log2(e) / T and 1 / T, each as the sum of two floats; the difference of two logits
+// from which on the exponential is 0.
 struct Scale2 {
-  float hi = 0.0f, lo = 0.0f, inv = 0.0f, inv_lo = 0.0f;
+  float hi = 0.0f, lo = 0.0f, inv = 0.0f, inv_lo = 0.0f, low = 0.0f;
 };
 // Rows of logits and the token chosen in each.
 struct LogitRows {

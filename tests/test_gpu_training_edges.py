@@ -1,0 +1,97 @@
+"""The training operators on the device where a bound of the usual size would hide a fault: extreme
+temperatures, impossible sequences, exact sums, rows whose result is known in closed form, gradients
+of views, and PyTorch's other ways of running a backward pass.
+
+Tolerances are counted beside each test, in half steps of the result's type (EPS32 is float32's).
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import training_ref as ref
+from test_gpu_training import _close, _gen, _grad_tolerance, _packed, _step, _step_state
+from training_ref import EPS32, half_step, tiny
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def sk():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    import sinkslot_b200
+    sinkslot_b200.load_library()
+    return sinkslot_b200
+
+
+# ------------------------------------------------------------------ extreme temperatures
+def _entropy_step(sk, z, tokens, temperature, g, gh):
+    z = z.detach().requires_grad_()
+    lp, h = sk.token_logprobs(z, tokens, temperature=temperature, entropy=True)
+    grad, = torch.autograd.grad([lp, h], [z], [g, gh])
+    want_lp, want_h, *_ = ref.logprobs64(z.detach(), tokens, temperature)
+    want = ref.logprobs_grad64(z.detach(), tokens, g, gh, temperature)
+    return lp.detach(), h.detach(), grad, want_lp, want_h, want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [40, 5003, 40000])
+@pytest.mark.parametrize("temperature,outer", [(1e-30, 1e-30), (1e-12, 1e-12), (2e-9, 1e-9),
+                                               (1e-4, 1e-4), (0.01, 1e-3)])
+def test_entropy_gradient_at_low_temperatures(sk, temperature, outer, vocab, dtype):
+    """Switched-off logits (-inf, or the type's lowest value) get a gradient of 0 at any temperature,
+    in rows with and without an outer gradient of the entropy."""
+    gen = _gen(vocab)
+    z = torch.randint(-6, 1, (8, vocab), generator=gen, device="cuda").to(dtype)
+    z[:, 0] = 0.0
+    z[:4, 5:9] = -math.inf
+    z[2:6, 9:14] = torch.finfo(dtype).min
+    z[6, 1:] = -math.inf
+    z[7, 1:] = torch.finfo(dtype).min
+    tokens = torch.zeros(8, dtype=torch.int64, device="cuda")
+    g = outer * torch.randn(8, generator=gen, device="cuda")
+    gh = outer * torch.randn(8, generator=gen, device="cuda")
+    gh[1] = 0.0
+    lp, h, grad, want_lp, want_h, want = _entropy_step(sk, z, tokens, temperature, g, gh)
+    _close(lp, want_lp, ref.logp_tolerance(z, tokens, temperature, vocab), "logp")
+    _close(h, want_h, 4 * (ref.sum_error(vocab) + 8 * EPS32) * (math.log(vocab + 1.0) + 1.0),
+           "entropy")
+    _close(grad, want, _grad_tolerance(z, tokens, g, gh, temperature, want, dtype), "grad")
+    off = z < -6
+    assert off.any() and not grad[off].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_entropy_gradient_under_a_loss_scale(sk, dtype):
+    """Masked logits, T = 0.01 and an outer gradient of 2^17: the product of both scales and the mask
+    must not reach infinity."""
+    gen = _gen(5)
+    z = torch.randn(6, 3001, generator=gen, device="cuda").to(dtype)
+    z[:, 2000:] = -math.inf
+    z[3:, 2000:] = torch.finfo(dtype).min
+    tokens = torch.randint(0, 2000, (6,), generator=gen, device="cuda")
+    g = torch.full((6,), 2.0 ** 17, device="cuda")
+    *_, grad, _, _, want = _entropy_step(sk, z, tokens, 0.01, g, g)
+    # a term under 2^-126 flushes to 0 before it is multiplied by at most (g + gh (|log p| + H)) / T
+    # (its sum is 1 or more; log p is over -104 - ln 3001 there and H under ln 3001)
+    flushed = 2.0 ** -126 * 2.0 ** 17 / 0.01 * (1 + 104 + 2 * math.log(3001))
+    _close(grad, want, _grad_tolerance(z, tokens, g, g, 0.01, want, dtype) + flushed, "grad")
+    assert not grad[:, 2000:].any()
+
+
+def test_entropy_of_far_logits_at_a_high_temperature(sk):
+    """Differences of many times 1e30 count as what they are where T is 1e30."""
+    z = torch.tensor([[0.0, -2e30, -5e30, -1e31, -math.inf, -3e38]], device="cuda").repeat(3, 700)
+    tokens = torch.tensor([1, 2, 6], device="cuda")
+    g = torch.tensor([1e30, -1e30, 2e30], device="cuda")
+    lp, h, grad, want_lp, want_h, want = _entropy_step(sk, z, tokens, 1e30, g, g)
+    vocab = z.shape[1]
+    _close(lp, want_lp, ref.logp_tolerance(z, tokens, 1e30, vocab), "logp")
+    _close(h, want_h, 4 * (ref.sum_error(vocab) + 8 * EPS32) * (math.log(vocab + 1.0) + 1.0),
+           "entropy")
+    _close(grad, want, _grad_tolerance(z, tokens, g, g, 1e30, want, z.dtype), "grad")
