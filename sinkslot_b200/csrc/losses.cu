@@ -371,8 +371,9 @@ __device__ __forceinline__ void preference_end(const double2* part, int64_t pair
       const double u = exp(-fabs(h));           // sigma(-|h|) = u / (1 + u)
       const double soft = log1p(u);
       const double neg = (h > 0.0 ? u : 1.0) / (1.0 + u), pos = (h > 0.0 ? 1.0 : u) / (1.0 + u);
-      each = (1.0 - smoothing) * (soft + (h < 0.0 ? -h : 0.0)) +
-             smoothing * (soft + (h > 0.0 ? h : 0.0));
+      each = (1.0 - smoothing) * (soft + (h < 0.0 ? -h : 0.0));
+      // (without smoothing its term is nothing, also where h is inf)
+      if (smoothing > 0.0) each += smoothing * (soft + (h > 0.0 ? h : 0.0));
       if (h != h) each = h;
       d = smoothing * pos - (1.0 - smoothing) * neg;
     } else if (kind == 1) {

@@ -95,3 +95,30 @@ def test_entropy_of_far_logits_at_a_high_temperature(sk):
     _close(h, want_h, 4 * (ref.sum_error(vocab) + 8 * EPS32) * (math.log(vocab + 1.0) + 1.0),
            "entropy")
     _close(grad, want, _grad_tolerance(z, tokens, g, g, 1e30, want, z.dtype), "grad")
+
+
+# ------------------------------------------------------------------ preference
+def test_preference_impossible_sequences(sk):
+    """A rejected sequence of probability 0 costs its pair nothing; a chosen one costs everything,
+    and with label smoothing either does."""
+    inf = math.inf
+    off = torch.arange(5, device="cuda")
+
+    def run(values, **kw):
+        logp = torch.tensor(values, device="cuda", requires_grad=True)
+        r = sk.preference_loss(logp, off, beta=0.5, **kw)
+        return r, torch.autograd.grad(r.loss, [logp])[0].tolist()
+
+    r, grad = run([-1.0, -2.0, -inf, -2.0])  # pairs (0, 2) and (1, 3)
+    # half of ln 2, rounded once from fp64
+    assert abs(float(r.loss.detach()) - math.log(2) / 2) <= EPS32
+    assert grad == [0.0, -0.125, 0.0, 0.125]
+    assert r.rejected_rewards.tolist() == [-inf, -1.0]
+    r, grad = run([-inf, -2.0, -1.0, -2.0])
+    assert float(r.loss.detach()) == inf and grad == [-0.25, -0.125, 0.25, 0.125]
+    r, _ = run([-1.0, -2.0, -inf, -2.0], label_smoothing=0.25)
+    assert float(r.loss.detach()) == inf
+    r, grad = run([-1.0, -2.0, -inf, -2.0], kind="hinge")
+    assert float(r.loss.detach()) == 0.5 and grad == [0.0, -0.25, 0.0, 0.25]
+    r, _ = run([-inf, -2.0, -inf, -2.0])
+    assert r.loss.isnan()
