@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/sinkslot_b200.h"
@@ -57,13 +58,18 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
   return at::empty({bytes}, like.options().dtype(at::kByte));
 }
 
-// An uninitialised (rows, vocab) tensor for the gradient of z: laid out as z is
-// (a view of a padded buffer gets rows as far apart, beginning on the same
-// 16-byte phase), contiguous where the rows of z overlap.
+// An uninitialised (rows, vocab) tensor for the gradient of z: rows beginning on the
+// same 16-byte phases as those of z (then both are read and written in whole vectors),
+// contiguous where the rows of z overlap.  Rows of a padded buffer are as far apart as
+// there; rows of a wider view (the last position of each sequence, every eighth row)
+// only as far as the phase asks: their own distance would be memory of the buffer's size.
 Tensor grad_like(const Tensor& z) {
-  const int64_t rows = z.size(0), vocab = z.size(1);
+  const int64_t rows = z.size(0), vocab = z.size(1), lanes = 16 / z.element_size();
   int64_t stride = z.stride(0);
-  if (stride < vocab || rows <= 1) stride = vocab;
+  if (stride < vocab || rows <= 1)
+    stride = vocab;
+  else if (stride - vocab > std::max<int64_t>(vocab / 8, 256))
+    stride = vocab + (stride - vocab) % lanes;
   const int64_t phase =
       rows ? (int64_t)(reinterpret_cast<uintptr_t>(z.const_data_ptr()) % 16) / z.element_size() : 0;
   if (stride == vocab && phase == 0) return at::empty({rows, vocab}, z.options());

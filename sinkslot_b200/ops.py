@@ -137,11 +137,14 @@ def _f32(like, *shape):
 
 
 def _grad_like(z):
-    """Rows as far apart as the logits' own, contiguous where those overlap."""
+    """Rows as far apart as a padded buffer's, by the least that keeps their 16-byte phases where
+    they lie further apart, contiguous where they overlap."""
     rows, vocab = z.shape
     stride = z.stride(0)
     if rows <= 1 or stride < vocab:
         stride = vocab
+    elif stride - vocab > max(vocab // 8, 256):
+        stride = vocab + (stride - vocab) % (16 // z.element_size())
     return torch.empty_strided((rows, vocab), (stride, 1), dtype=z.dtype, device=z.device)
 
 

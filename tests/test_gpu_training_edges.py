@@ -122,3 +122,36 @@ def test_preference_impossible_sequences(sk):
     assert float(r.loss.detach()) == 0.5 and grad == [0.0, -0.25, 0.0, 0.25]
     r, _ = run([-inf, -2.0, -inf, -2.0])
     assert r.loss.isnan()
+
+
+# ------------------------------------------------------------------ gradients of views
+def test_gradient_of_rows_far_apart_takes_its_own_size(sk):
+    """The last position of each sequence, and every eighth row: the gradient is as large as the
+    logits it belongs to, not as the buffer they are seen in."""
+    gen = _gen(9)
+    full = torch.randn(6, 64, 1003, generator=gen, device="cuda").bfloat16()
+    tokens = torch.randint(0, 1003, (6,), generator=gen, device="cuda")
+    old = torch.full((6,), -7.0, device="cuda")
+    for z in (full[:, -1], full[:, 3, 1:1001], full[0, ::8][:6], full[:, 0, :5]):
+        t = tokens % z.shape[1]
+        want = None
+        for leaf in (z.detach().clone(), z.detach()):
+            leaf.requires_grad_()
+            a, = torch.autograd.grad(sk.token_logprobs(leaf, t).sum(), [leaf])
+            r = sk.policy_loss_from_logits(leaf, t, old, old)
+            b, = torch.autograd.grad(r.loss, [leaf])
+            if want is None:
+                want = a, b
+            # (rows on another phase are added up in another order: a few steps of float32 before
+            # the rounding to 16 bits, so at most one step of those)
+            torch.testing.assert_close(a, want[0], rtol=2 * half_step(a.dtype) * 2, atol=1e-6)
+            torch.testing.assert_close(b, want[1], rtol=2 * half_step(a.dtype) * 2, atol=1e-6)
+            for grad in (a, b):
+                assert grad.shape == z.shape
+                assert grad.untyped_storage().nbytes() <= 2 * (z.shape[0] * (z.shape[1] + 264))
+                assert (grad.data_ptr() - leaf.data_ptr()) % 16 == 0
+                if z.shape[0] > 1:
+                    assert (grad.stride(0) - leaf.stride(0)) * 2 % 16 == 0
+    padded = torch.randn(9, 1003 + 61, generator=gen, device="cuda")[:, :1003].requires_grad_()
+    grad, = torch.autograd.grad(sk.token_logprobs(padded, tokens.repeat(2)[:9]).sum(), [padded])
+    assert grad.stride() == padded.stride()  # a padded buffer keeps its rows' distance

@@ -58,3 +58,21 @@ def test_forward_mode_is_refused(fake):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (_cuda(*shape),), (_cuda(*shape),))
         call(_cuda(*shape))
+
+
+def test_fake_gradients_lie_as_the_real_ones(fake):
+    """Rows of a padded buffer keep their distance; rows far apart come together."""
+    grad = torch.ops.sinkslot_b200.token_logprobs_grad.default
+    ids, v = _cuda(8, dtype=torch.int64), _cuda(8)
+
+    def stride(z):
+        return grad(z, ids, _cuda(8, 2), v, v, None, 1.0, -100).stride()
+
+    for dtype, lanes in ((torch.float32, 4), (torch.bfloat16, 8)):
+        wide = _cuda(8, 8192, 1003, dtype=dtype)
+        apart = 8192 * 1003 - 1003
+        assert stride(wide[:, -1]) == (1003 + apart % lanes, 1)
+        assert stride(_cuda(8, 1003 + 256, dtype=dtype)[:, :1003]) == (1003 + 256, 1)
+        assert stride(_cuda(8, 1003 + 257, dtype=dtype)[:, :1003]) == (1003 + 257 % lanes, 1)
+        assert stride(_cuda(8, 9000, dtype=dtype)[:, :8000]) == (9000, 1)
+        assert stride(_cuda(1, 1003, dtype=dtype).expand(8, 1003)) == (1003, 1)
