@@ -184,7 +184,12 @@ def torch_ops():
                 raise ImportError(
                     f"{TORCH_LIB_PATH} is missing: the training operators must be built "
                     f"(python -m sinkslot_b200.build); sinkslot_b200 has no fallback")
-            torch.ops.load_library(TORCH_LIB_PATH)
+            try:
+                torch.ops.load_library(TORCH_LIB_PATH)
+            except OSError as e:
+                raise ImportError(
+                    f"{TORCH_LIB_PATH} does not load ({e.__cause__ or e}): the training operators "
+                    f"must be built for the installed torch (python -m sinkslot_b200.build)") from e
             from . import ops
             ops.register_training_fakes()
             ns = torch.ops.sinkslot_b200
@@ -195,6 +200,11 @@ def torch_ops():
 
 
 def load_library():
-    """Loads both libraries now; the C ABI's binding is returned."""
-    torch_ops()
-    return lib()
+    """Loads what is built now; the C ABI's binding is returned.  Raises if libsinkslot_b200.so is
+    missing; training operators that are missing raise where they are called."""
+    binding = lib()
+    try:
+        torch_ops()
+    except ImportError:
+        pass
+    return binding
