@@ -38,7 +38,7 @@ from .losses import (
     policy_loss_from_logits,
     preference_loss,
 )
-from ._lib import LIB_PATH, SinkslotError, load_library
+from ._lib import LIB_PATH, SinkslotError, current, load_library
 
 __all__ = [
     "get_random_projections",
@@ -70,7 +70,11 @@ __all__ = [
     "load_library",
 ]
 
-try:  # registers the training operators too, where they are built (else at the first use)
-    load_library()
-except (ImportError, OSError):
-    pass
+# Registers the training operators where they are built from these sources, else their first use
+# does: a build that follows must not find older libraries in the process.
+if current():
+    try:
+        load_library()
+    except (ImportError, OSError):
+        pass
+del current

@@ -8,6 +8,7 @@ library is an error: there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import glob
 import os
 import threading
 import types
@@ -18,8 +19,11 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsinkslot_b200.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "libsinkslot_b200_torch.so")
 
+ABI = 102  # sinkslot_abi_version() of the library that this binding is for
+
 _lock = threading.Lock()
 _lib = None
+_opened = False  # a library of this package is in the process, used or refused
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
@@ -116,8 +120,9 @@ class SinkslotError(RuntimeError):
 
 
 def lib():
-    """The loaded library; raises if it is missing (no fallback exists)."""
-    global _lib
+    """The loaded library; raises if it is missing, or was built from other sources (no fallback
+    exists)."""
+    global _lib, _opened
     if _lib is not None:
         return _lib
     with _lock:
@@ -128,16 +133,44 @@ def lib():
                 f"{LIB_PATH} is missing: the sm_100a extension must be built "
                 f"(python -m sinkslot_b200.build); sinkslot_b200 has no CPU or library fallback")
         L = ctypes.CDLL(LIB_PATH)
-        for name, argtypes in _SIGNATURES.items():
-            fn = getattr(L, name)
-            fn.argtypes = argtypes
-            fn.restype = c_int
-        L.sinkslot_last_error.argtypes = []
-        L.sinkslot_last_error.restype = ctypes.c_char_p
-        L.sinkslot_abi_version.argtypes = []
-        L.sinkslot_abi_version.restype = c_int
+        _opened = True
+        try:
+            L.sinkslot_abi_version.argtypes = []
+            L.sinkslot_abi_version.restype = c_int
+            abi = L.sinkslot_abi_version()
+            if abi != ABI:
+                raise ImportError(f"{LIB_PATH} has ABI {abi}, this package needs {ABI}: it was "
+                                  f"built from other sources (python -m sinkslot_b200.build)")
+            for name, argtypes in _SIGNATURES.items():
+                fn = getattr(L, name)
+                fn.argtypes = argtypes
+                fn.restype = c_int
+            L.sinkslot_last_error.argtypes = []
+            L.sinkslot_last_error.restype = ctypes.c_char_p
+        except AttributeError as e:
+            raise ImportError(f"{e}: the library was built from other sources "
+                              f"(python -m sinkslot_b200.build)") from e
         _lib = L
     return _lib
+
+
+def current() -> bool:
+    """Whether both libraries are there and no older than their sources."""
+    def newest(*patterns):
+        return max((os.path.getmtime(f) for p in patterns
+                    for f in glob.glob(os.path.join(_HERE, *p))), default=0.0)
+
+    header = ("..", "include", "*.h")
+    try:
+        return (os.path.getmtime(LIB_PATH) >= newest(("csrc", "*.cu"), ("csrc", "*.cuh"),
+                                                     ("csrc", "*.h"), header)
+                and os.path.getmtime(TORCH_LIB_PATH) >= newest(("csrc", "*.cpp"), header))
+    except OSError:
+        return False
+
+
+def opened() -> bool:
+    return _opened
 
 
 def call(name: str, *args) -> None:

@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -46,6 +47,15 @@ def _headers_mtime() -> float:
     return max((os.path.getmtime(h) for h in hs), default=0.0)
 
 
+def _replace(new: str, path: str) -> None:
+    """Puts a built library in its place.  What a process has loaded stays loaded."""
+    os.replace(new, path)
+    from . import _lib
+    if _lib.opened():
+        warnings.warn(f"{os.path.basename(path)} was built while an older one is loaded: it is "
+                      f"used from a new process on", RuntimeWarning, stacklevel=3)
+
+
 def _build_torch_ops(verbose: bool) -> None:
     """libsinkslot_b200_torch.so, when its source, the C header or torch changed."""
     import torch
@@ -70,7 +80,7 @@ def _build_torch_ops(verbose: bool) -> None:
         sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for csrc/torch_ops.cpp")
-    os.replace(tmp, TORCH_LIB)
+    _replace(tmp, TORCH_LIB)
     with open(stamp, "w") as f:
         f.write(torch.__version__)
 
@@ -107,7 +117,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
             raise RuntimeError("link of libsinkslot_b200.so failed")
-        os.replace(tmp, LIB)
+        _replace(tmp, LIB)
     _build_torch_ops(verbose)
     return LIB
 
