@@ -168,3 +168,32 @@ with warnings.catch_warnings(record=True) as seen:
 print(*[w.message for w in seen if "new process" in str(w.message)])
 """, **_compilers(copy))
     assert "sinkslot_b200::lookup" in out and "new process" in out
+
+
+def test_build_gives_the_solver_where_the_bindings_do_not_compile(copy):
+    """The solver's library is built and loads; the bindings of other sources are taken away, and
+    the build command fails."""
+    env = _compilers(copy)
+    tools = copy / "tools"
+    _age(copy, TORCH_LIB)
+    _script(tools / "g++", "#!/bin/sh\necho no torch headers >&2\nexit 1\n")
+    out = _python(copy, USE + """
+import os, warnings
+import sinkslot_b200 as sk
+from sinkslot_b200 import build
+with warnings.catch_warnings(record=True) as seen:
+    warnings.simplefilter("always")
+    assert build.build() == sk.LIB_PATH
+print(*[w.message for w in seen])
+assert sk.load_library().sinkslot_abi_version() >= 102
+assert not os.path.exists(build.TORCH_LIB)
+try:
+    use(sk)
+except ImportError as e:
+    print("raised", e)
+""", **env)
+    assert "training operators" in out and "raised" in out
+    r = subprocess.run([sys.executable, "-m", "sinkslot_b200.build"], cwd=copy,
+                       env={**os.environ, "PYTHONPATH": str(copy), **env}, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode != 0 and "no torch headers" in r.stderr
