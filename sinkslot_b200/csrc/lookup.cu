@@ -608,8 +608,10 @@ __device__ __forceinline__ void put_sum(const SumArgs& a, T* out, bool head, int
 // kAligned: all rows of both arrays begin on 16-byte boundaries.  The windows'
 // keys and positions are staged in shared memory where a CTA meets few windows
 // (ncv of kStageFrom or more).  Registers are held to 64 for four CTAs on an SM
-// (5003 x 771 fp16, 40009 tokens, sort and all: 87 us at three, 73 at four, 89 at five,
-// which spill).
+// (5003 x 771 fp16, 40009 tokens, sort and all: 87 us at three, 73 at four, 89 at five).
+// The vector variants spill at four already (staged, 16-bit types: 112 bytes stored and
+// 132 loaded for each thread on any alignment, 44 and 104 aligned; float32: 28 and 24,
+// 36 and 96).
 constexpr int kStageFrom = 64;
 constexpr int kStaged = (kLookThreads / kStageFrom + 1) * 64;
 

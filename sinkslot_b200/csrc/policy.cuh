@@ -30,7 +30,10 @@ struct TokenTerm {
 };
 
 // One token's loss, KL estimate and d loss / d logp.  The clip is decided on the
-// difference of the log-probabilities in fp64, which is exact.
+// difference of the log-probabilities in fp64, which is exact.  The ratio, the KL term
+// and the coefficient are float32 (as the log-probabilities and the result are; a
+// token's loss is good to a few steps, and the sums over tokens are fp64): over 16384
+// tokens the outputs are 7e-8 of their size off where fp64 terms, rounded once, are 3e-8.
 __device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const PolicyEdges& e,
                                                  float logp, float old_logp, float ref_logp,
                                                  float adv) {

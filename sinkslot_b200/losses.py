@@ -50,8 +50,9 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
     (sequences that count no token are left out).
 
     ``logp``, ``old_logp``, ``ref_logp``: float32, (tokens,).  ``advantages``:
-    float32, one per token, else one per sequence.  ``mask``: bool; False leaves
-    a token out.  ``offsets``: int32 or int64, (sequences + 1,), non-decreasing;
+    float32, one per token, else one per sequence (as many as there are tokens
+    are one per token, whatever the sequences).  ``mask``: bool; False leaves a
+    token out.  ``offsets``: int32 or int64, (sequences + 1,), non-decreasing;
     without it all tokens are one sequence.  Tokens outside the sequences are not
     counted and get a gradient of 0.  Differentiable in ``logp``.
     """
@@ -79,7 +80,10 @@ def policy_loss_from_logits(logits: torch.Tensor, tokens: torch.Tensor, old_logp
     once.  It is made for a loss multiplied by ``grad_scale``: where the outer
     gradient is just that (1, or the factor of a loss scaler) the backward pass
     hands it over as it is; any other outer gradient costs a pass that scales it
-    and rounds it a second time.
+    and rounds it a second time.  So pass ``grad_scale=1 / n`` for
+    ``(loss / n).backward()``, and a loss scaler's factor with float16 logits,
+    whose gradient's smallest elements are lost before a later factor could save
+    them.  Saved-tensor hooks do not see this gradient.
     """
     return PolicyLossResult(*torch_ops().policy_from_logits(
         logits, tokens, old_logp, advantages, temperature, ref_logp, mask, offsets, clip_low,
