@@ -44,8 +44,9 @@ __device__ __forceinline__ TokenTerm policy_term(const PolicyTerms& t, const Pol
   const float rc = over ? e.rhi : (under ? e.rlo : r);
   // min(r A, clip(r) A) is the clipped one where r is outside on A's side
   o.clipped = adv > 0.0f ? over : (adv < 0.0f ? under : false);
-  o.loss = -(o.clipped ? rc : r) * adv;
-  o.coef = o.clipped ? 0.0f : -r * adv;
+  const float ra = adv == 0.0f && d < INFINITY ? 0.0f : r * adv;  // r may be past float32
+  o.loss = o.clipped ? -rc * adv : -ra;
+  o.coef = o.clipped ? 0.0f : -ra;
   o.kl = 0.0f;
   if (t.ref_logp) {
     const float g = (float)((double)ref_logp - (double)logp);

@@ -317,6 +317,30 @@ def test_policy_from_logits_scales_its_gradient(sk, t, vocab, off, pad, dtype):
                      average="token", outer=outer)
 
 
+@pytest.mark.parametrize("t,vocab", [(40, 1003), (5600, 13001)])  # three passes; one pass
+def test_tokens_without_advantage_count_nothing_at_any_ratio(sk, t, vocab):
+    """A = 0 (a group of equal rewards): r A is 0 also where r = e^190 is past float32."""
+    gen = _gen(t)
+    z = torch.randn(t, vocab, generator=gen, device="cuda").half().requires_grad_()
+    tokens = torch.randint(0, vocab, (t,), generator=gen, device="cuda")
+    lp = sk.token_logprobs(z, tokens)
+    adv = torch.ones(t, device="cuda")
+    old = lp.detach().clone()
+    adv[::3] = 0.0
+    old[::3] -= 190.0
+    want = -adv.double().mean()  # ratios of 1, rounded nowhere
+    coef = (-adv / t).requires_grad_(False)
+    wgrad, = torch.autograd.grad(lp, [z], coef, retain_graph=True)
+    split = sk.policy_loss(lp, old, adv)
+    fused = sk.policy_loss_from_logits(z, tokens, old, adv)
+    for r in (split, fused):
+        # (the fused pass may round a log-probability of 12 or less to the step beside old's)
+        assert abs(float(r.loss.detach()) - float(want)) <= 16 * EPS32
+        grad, = torch.autograd.grad(r.loss, [z], retain_graph=r is split)
+        torch.testing.assert_close(grad, wgrad, rtol=2 * half_step(z.dtype) * 2, atol=2 * tiny(z.dtype) * 2)
+        assert not grad[::3].any()
+
+
 # ------------------------------------------------------------------ other ways through autograd
 def test_saved_tensor_hooks(sk):
     """What is saved for the backward pass, moved to the host and back: the same gradients."""
